@@ -181,3 +181,22 @@ def stream_ptr(stream=None) -> int:
 
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
+
+
+def require_current_device(what: str, *tensors):
+    """Raises ``ValueError`` unless every tensor (``None`` is skipped) lies on the current CUDA device: kernels are launched on the
+    current device's stream."""
+    index = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{what}: operand on {t.device}, the current device is cuda:{index}")
+
+
+def run_on_stream(stream, tensors, fn):
+    """``fn()`` with ``stream`` as the current stream: what it allocates belongs to that stream, and the operands ``tensors`` (``None``
+    is skipped) are marked as used there."""
+    for t in tensors:
+        if t is not None and t.is_cuda:
+            t.record_stream(stream)
+    with torch.cuda.stream(stream):
+        return fn()

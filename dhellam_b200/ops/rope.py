@@ -1,13 +1,19 @@
-"""Rotary position embedding applied in place to the Q and K heads of a packed QKV buffer.
+"""Rotary position embedding.
 
 The reference uses learned absolute positions (dhellam/core/dshb.py:250-255); RoPE is
-needed for the Llama family.  Layout of one row of ``qkv``:
-``[nq heads x d | nkv heads x d | nkv heads x d]``; pairs are ``(i, i + d/2)``.
+needed for the Llama family.  Two forms:
+
+* ``rope_apply_`` rotates the Q and K heads of a packed QKV buffer in place, whole heads with pairs ``(i, i + d/2)`` and
+  angles from a table (``rope_table``).  Layout of one row of ``qkv``: ``[nq heads x d | nkv heads x d | nkv heads x d]``.
+* ``rope_fwd`` / ``rope_bwd`` rotate separate (strided) queries and keys, out of place or in place: pairs in halves or
+  interleaved, the whole head or its first part, any position, frequencies from ``rope_frequencies``, which also states
+  the ways in which models are stretched to longer contexts than they were first trained on.
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_void_p
-from functools import lru_cache
+import math
+from ctypes import c_float, c_int, c_int64, c_void_p
+from dataclasses import dataclass
 
 import torch
 
@@ -44,3 +50,144 @@ def rope_apply_(qkv, positions, cos, sin, nq: int, nkv: int, d: int, inverse: bo
     K.check(fn(qkv.data_ptr(), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), T, qkv.stride(0), nq + nkv, d,
                1 if inverse else 0, sm_budget, K.stream_ptr(stream)), "dh_rope_inplace")
     return qkv
+
+
+# ----------------------------------------------------------------------------- separate heads, other layouts, longer contexts
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the frequencies of a model first trained on ``original_max_position`` positions are stretched ``factor`` times.
+
+    * ``linear``: every frequency divided by ``factor`` (positions interpolated);
+    * ``ntk``: the base raised so that the slowest pair is divided by ``factor`` and the fastest stays;
+    * ``llama3``: pairs that turn at least ``high_freq_factor`` times within the original length stay, pairs that turn at most
+      ``low_freq_factor`` times are divided by ``factor``, linear in the number of turns in between;
+    * ``yarn``: the same with a ramp over the pair's index between the pairs of ``beta_fast`` and ``beta_slow`` turns, and
+      cosines and sines multiplied by ``attention_factor`` (default ``0.1 ln(factor) + 1``)."""
+    kind: str = "linear"
+    factor: float = 1.0
+    original_max_position: int = 8192
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "llama3", "yarn"):
+            raise ValueError(f"unknown rotary scaling {self.kind!r}: linear, ntk, llama3 or yarn")
+        if not self.factor >= 1.0 or self.original_max_position <= 0:
+            raise ValueError("rotary scaling needs a factor of at least 1 and a positive original length")
+        if self.kind == "llama3" and not self.high_freq_factor > self.low_freq_factor > 0:
+            raise ValueError("llama3 scaling needs high_freq_factor > low_freq_factor > 0")
+        if self.kind == "yarn" and not self.beta_fast > self.beta_slow > 0:
+            raise ValueError("yarn scaling needs beta_fast > beta_slow > 0")
+
+
+def rope_frequencies(rotary_dim: int, theta: float, scaling: RopeScaling | None = None, device="cpu"):
+    """``(frequencies [rotary_dim / 2] fp64, scale)``: radians per position of every pair, and the factor on cosines and sines."""
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError(f"the rotated part of a head has an even number of elements, not {rotary_dim}")
+    i = torch.arange(0, rotary_dim, 2, dtype=torch.float64) / rotary_dim
+    freq, scale = float(theta) ** -i, 1.0
+    s = scaling
+    if s is not None and s.kind == "linear":
+        freq = freq / s.factor
+    elif s is not None and s.kind == "ntk":
+        freq = (float(theta) * s.factor ** (rotary_dim / max(rotary_dim - 2, 1))) ** -i
+    elif s is not None and s.kind == "llama3":
+        turns = s.original_max_position * freq / (2 * math.pi)
+        keep = ((turns - s.low_freq_factor) / (s.high_freq_factor - s.low_freq_factor)).clamp(0.0, 1.0)
+        freq = freq * keep + freq / s.factor * (1.0 - keep)
+    elif s is not None:
+        def index_of(turns):                 # the (fractional) pair that turns so often within the original length
+            return rotary_dim * math.log(s.original_max_position / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        lo = max(math.floor(index_of(s.beta_fast)), 0)
+        hi = min(math.ceil(index_of(s.beta_slow)), rotary_dim - 1)
+        ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0.0, 1.0)
+        freq = freq / s.factor * ramp + freq * (1.0 - ramp)
+        scale = s.attention_factor if s.attention_factor is not None else 0.1 * math.log(s.factor) + 1.0
+    return freq.to(device), scale
+
+
+def _turn_ref(x, positions, freq, interleaved, scale, transposed):
+    r = 2 * freq.numel()
+    angle = positions.to(torch.float64).unsqueeze(-1) * freq.to(torch.float64)
+    cos, sin = (angle.cos() * scale).float().unsqueeze(-2), (angle.sin() * scale).float().unsqueeze(-2)
+    if transposed:
+        sin = -sin
+    y = x.float().clone()
+    a, b = (y[..., 0:r:2], y[..., 1:r:2]) if interleaved else (y[..., : r // 2], y[..., r // 2:r])
+    c, d = a * cos - b * sin, b * cos + a * sin
+    a.copy_(c), b.copy_(d)
+    return y.to(x.dtype)
+
+
+def _heads_fit(x, lead, d, dtype):
+    return x.dim() in (3, 4) and x.shape[:-2] == lead and x.shape[-1] == d and x.dtype == dtype and (x.stride(-1) == 1 or d == 1)
+
+
+def _strides(x):
+    return (x.stride(0), 0, x.stride(1)) if x.dim() == 3 else (x.stride(0), x.stride(1), x.stride(2))
+
+
+def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget, stream, what):
+    if stream is not None:
+        operands = (q, k, positions, freq) + (tuple(out) if out is not None else ())
+        return K.run_on_stream(stream, operands, lambda: _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
+                                                               None, what))
+    lead, d = q.shape[:-2], q.shape[-1]
+    pairs = [(q, out[0] if out is not None else None)] + ([(k, out[1] if out is not None else None)] if k is not None else [])
+    if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: one int32 or int64 position for each of {tuple(lead)} rows, got {positions.dtype} {tuple(positions.shape)}")
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not 0 < 2 * freq.numel() <= d:
+        raise ValueError(f"{what}: fp64 frequencies of at most half of the {d} elements of a head, got {freq.dtype} {tuple(freq.shape)}")
+    for x, o in pairs:
+        if not _heads_fit(x, lead, d, q.dtype):
+            raise ValueError(f"{what}: queries and keys are [rows..., heads, {d}] of one type, with elements side by side")
+        if o is None:
+            continue
+        if o.shape != x.shape or not _heads_fit(o, lead, d, q.dtype):
+            raise ValueError(f"{what}: an output has its input's shape and type, with elements side by side")
+        in_place = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+        if not in_place and any(o.untyped_storage().data_ptr() == y.untyped_storage().data_ptr() for y, _ in pairs):
+            raise ValueError(f"{what}: an output is its own input or shares no memory with the inputs")
+        if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+            raise ValueError(f"{what}: an output has room for every row and head")
+    if out is not None and k is not None and out[0].data_ptr() == out[1].data_ptr() and q.numel() and k.numel():
+        raise ValueError(f"{what}: queries and keys have outputs of their own")
+    if not K.use_native(q):
+        res = [_turn_ref(x, positions, freq, interleaved, scale, transposed) for x, _ in pairs]
+        res = [r if o is None else o.copy_(r) for r, (_, o) in zip(res, pairs)]
+        return res[0], (res[1] if k is not None else None)
+    if q.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what}: the sm_100a kernel rotates bf16 and fp32, not {q.dtype}")
+    K.require_current_device(what, q, k, positions, freq, *(out or ()))
+    if not positions.is_contiguous() or not freq.is_contiguous():
+        raise ValueError(f"{what}: positions and frequencies must be contiguous")
+    pairs = [(x, torch.empty(x.shape, dtype=x.dtype, device=x.device) if o is None else o) for x, o in pairs]
+    ptrs, strides = (c_void_p * 4)(), (c_int64 * 12)()
+    for i, (x, o) in enumerate(pairs):
+        ptrs[2 * i], ptrs[2 * i + 1] = x.data_ptr(), o.data_ptr()
+        strides[6 * i:6 * i + 6] = _strides(x) + _strides(o)
+    fn = K.proto("dh_rope_heads", [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int,
+                                   c_float, c_int, c_int, c_void_p])
+    K.check(fn(ptrs, strides, q.shape[-2], 0 if k is None else k.shape[-2], positions.data_ptr(), int(positions.dtype == torch.int64),
+               freq.data_ptr(), positions.numel(), 1 if len(lead) == 1 else max(lead[1], 1), d, 2 * freq.numel(), int(bool(interleaved)),
+               int(q.dtype == torch.float32), scale, int(transposed), sm_budget, K.stream_ptr()), "dh_rope_heads")
+    return pairs[0][1], (pairs[1][1] if k is not None else None)
+
+
+def rope_fwd(q, k, positions, freq, interleaved: bool = False, scale: float = 1.0, out=None, sm_budget: int = 0, stream=None):
+    """Rotated queries and keys ``(q', k')``.
+
+    ``q [T, Hq, d]`` and ``k [T, Hk, d]`` (packed rows, as ``pymha_varlen_fwd`` takes them) or ``[S, B, heads, d]`` (as
+    ``attn_fwd`` does), bf16 or fp32, any strides with the elements of a head side by side; ``k`` may be ``None``.
+    ``positions [T]`` (``[S, B]``) int32 or int64, any value.  ``freq [r / 2]`` fp64 and ``scale`` come from
+    ``rope_frequencies``: the first ``r`` elements of every head are rotated, as pairs ``(i, i + r/2)`` or, interleaved,
+    ``(2i, 2i + 1)``; the others are copied.  ``out = (q', k')`` names the outputs, which may be the inputs themselves."""
+    return _turn(q, k, positions, freq, interleaved, scale, out, False, sm_budget, stream, "rope_fwd")
+
+
+def rope_bwd(dq, dk, positions, freq, interleaved: bool = False, scale: float = 1.0, out=None, sm_budget: int = 0, stream=None):
+    """Gradients of the queries and keys that ``rope_fwd`` took, from those of what it gave: the transposed rotation, same arguments."""
+    return _turn(dq, dk, positions, freq, interleaved, scale, out, True, sm_budget, stream, "rope_bwd")
