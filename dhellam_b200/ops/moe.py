@@ -2,15 +2,16 @@
 
 New relative to the reference (it has no MoE ops; see ``models/moe.py``).  The router runs
 as one sm_100a kernel on CUDA tensors (csrc/head_optim.cu, ``router_kernel``: logits, softmax, top-k and gate
-normalisation in one pass over the token row); the plan and the permutations use index
+normalisation in one pass over the token row), and so do the balance loss with the per-expert counts and the gradient of
+gates and balance to the router's logits (csrc/balance.cu); the plan and the permutations use index
 arithmetic on the device, and the only host read is the per-expert row count that sizes
 the expert GEMMs (dropless routing has data-dependent shapes).
 """
 from __future__ import annotations
 
-from ctypes import c_int, c_void_p
+from ctypes import c_float, c_int, c_int64, c_void_p
 from dataclasses import dataclass
-from typing import List, Optional
+from typing import List, NamedTuple, Optional
 
 import torch
 import torch.distributed as dist
@@ -40,6 +41,64 @@ def router_topk_fwd(x, w, k: int):
     return probs, topi, gates
 
 
+class Balance(NamedTuple):
+    """What the backward of the balance loss needs."""
+    coef: torch.Tensor               # [E] fp32: gradient of the loss with respect to a counted token's probabilities
+    mask: Optional[torch.Tensor]     # [T] bool / uint8: the counted tokens (None: all)
+
+
+def _router_operands(what, probs, topi, mask):
+    if probs.dim() != 2 or topi.dim() != 2 or topi.shape[0] != probs.shape[0] or probs.dtype != torch.float32 \
+            or topi.dtype not in (torch.int32, torch.int64) or not topi.shape[1]:
+        raise ValueError(f"{what}: fp32 probabilities [T, E] and int32 or int64 choices [T, k], got {probs.dtype} {tuple(probs.shape)} "
+                         f"and {topi.dtype} {tuple(topi.shape)}")
+    if mask is not None and (mask.shape != probs.shape[:1] or mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"{what}: a mask of {probs.shape[0]} bool or uint8 values, got {mask.dtype} {tuple(mask.shape)}")
+
+
+def _on_kernel(probs, topi, *others):
+    """Whether the kernels of csrc/balance.cu take these operands.  Both functions were composed of PyTorch ops before and still are for
+    what only those handle: CPU tensors, the library backend, tensors that are differentiated, traced or on another device."""
+    return K.use_native(probs) and probs.shape[1] <= 1024 and K.is_plain(probs) and (probs.stride(1) == 1 or probs.shape[1] == 1) \
+        and all(t is None or (t.get_device() == probs.get_device() and K.is_plain(t)) for t in (topi, *others))
+
+
+def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
+    """Load-balancing loss ``E * sum_e f_e * P_e`` (fraction of the choices x mean probability) over the counted tokens.
+
+    ``probs [T, E]`` fp32 and ``topi [T, k]`` (int32 or int64) are the router's probabilities and choices, ``mask [T]`` (bool or
+    uint8) leaves out padding tokens.  A choice outside ``[0, E)`` counts for no expert.  Returns ``(loss, counts [E] int32,
+    balance)``: the loss is 0 where no token is counted, ``balance`` goes to ``router_topk_bwd``."""
+    if stream is not None:
+        return K.run_on_stream(stream, (probs, topi, mask), lambda: balance_loss_fwd(probs, topi, mask, sm_budget))
+    _router_operands("balance_loss_fwd", probs, topi, mask)
+    T, E = probs.shape
+    k = topi.shape[1]
+    if _on_kernel(probs, topi, mask):
+        if topi.stride(1) != 1:
+            topi = topi.contiguous()
+        if mask is not None and not mask.is_contiguous():
+            mask = mask.contiguous()
+        parts = K.proto("dh_balance_parts", [c_int, c_int, c_int])(T, E, sm_budget)
+        out = torch.empty(1 + 2 * E, dtype=torch.float32, device=probs.device)
+        loss, coef, counts = out[0], out[1:1 + E], out[1 + E:].view(torch.int32)
+        scratch = torch.empty(parts * (2 * E + 1), dtype=torch.float32, device=probs.device)
+        base = out.data_ptr()
+        fn = K.proto("dh_balance_fwd", [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
+                                        c_void_p, c_void_p, c_void_p, c_void_p])
+        K.check(fn(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), int(topi.dtype == torch.int64), K.ptr(mask), T, E, k,
+                   scratch.data_ptr(), parts, base, base + 4 * (1 + E), base + 4, K.stream_ptr()), "dh_balance_fwd")
+        return loss, counts, Balance(coef, mask)
+    counted = torch.ones(T, dtype=torch.bool, device=probs.device) if mask is None else mask != 0
+    n = counted.sum().clamp_min(1)
+    # an extra column takes the choices that count for nobody
+    used = torch.where((topi >= 0) & (topi < E) & counted[:, None], topi.long(), E).reshape(-1)
+    counts = torch.bincount(used, minlength=E + 1)[:E]
+    coef = counts.to(torch.float32) / n / n * (E / k)
+    loss = (coef * torch.where(counted[:, None], probs, torch.zeros_like(probs)).sum(0)).sum()
+    return loss, counts.to(torch.int32), Balance(coef, mask)
+
+
 def aux_loss(probs, topi, E: int):
     """Load-balancing loss ``E * sum_e f_e * P_e`` (fraction routed x mean probability)."""
     frac = torch.zeros(E, dtype=torch.float32, device=probs.device)
@@ -48,18 +107,44 @@ def aux_loss(probs, topi, E: int):
     return E * (frac * probs.mean(0)).sum()
 
 
-def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0):
-    """Gradient with respect to the router logits ``[T,E]`` (fp32)."""
-    T = probs.shape[0]
-    topv_sum = probs.gather(1, topi).sum(-1, keepdim=True)
-    d_topv = (d_gates - (d_gates * gates).sum(-1, keepdim=True)) / topv_sum
+def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0, balance: Optional[Balance] = None, sm_budget: int = 0,
+                    stream=None):
+    """Gradient with respect to the router logits ``[T,E]`` (fp32): of the gates (``d_gates [T,k]``) and, times ``aux_scale``, of the
+    balance loss.  ``balance`` comes from ``balance_loss_fwd``; without it all tokens count."""
+    if stream is not None:
+        operands = (d_gates, probs, topi, gates) + (tuple(balance) if balance is not None else ())
+        return K.run_on_stream(stream, operands, lambda: router_topk_bwd(d_gates, probs, topi, gates, E, aux_scale, balance, sm_budget))
+    mask = balance.mask if balance is not None else None
+    _router_operands("router_topk_bwd", probs, topi, mask)
+    if probs.shape[1] != E or d_gates.shape != topi.shape or gates.shape != topi.shape or (balance is not None and balance.coef.shape != (E,)):
+        raise ValueError(f"router_topk_bwd: gates and their gradient as the choices {tuple(topi.shape)}, probabilities and balance of {E} "
+                         f"experts")
+    T, k = topi.shape
+    if _on_kernel(probs, topi, d_gates, gates, mask) and d_gates.dtype == gates.dtype == torch.float32:
+        if aux_scale and balance is None:
+            balance = balance_loss_fwd(probs, topi)[2]
+        topi, gates, d_gates = (t if t.stride(1) == 1 else t.contiguous() for t in (topi, gates, d_gates))
+        out = torch.empty((T, E), dtype=torch.float32, device=probs.device)
+        fn = K.proto("dh_router_bwd", [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                       c_float, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
+        K.check(fn(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), int(topi.dtype == torch.int64), K.ptr(mask),
+                   gates.data_ptr(), gates.stride(0), d_gates.data_ptr(), d_gates.stride(0), balance.coef.data_ptr() if aux_scale else 0,
+                   aux_scale, out.data_ptr(), T, E, k, sm_budget, K.stream_ptr()), "dh_router_bwd")
+        return out
+    valid = (topi >= 0) & (topi < E)
+    at = torch.where(valid, topi, torch.zeros_like(topi)).long()
+    topv_sum = torch.where(valid, probs.gather(1, at), 0.0).sum(-1, keepdim=True)
+    dg = torch.where(valid, d_gates, 0.0)
+    d_topv = torch.where(valid & (topv_sum != 0), (dg - (dg * gates).sum(-1, keepdim=True)) / topv_sum, 0.0)
     d_probs = torch.zeros_like(probs)
-    d_probs.scatter_add_(1, topi, d_topv)
+    d_probs.scatter_add_(1, at, d_topv)
     if aux_scale:
-        frac = torch.zeros(E, dtype=torch.float32, device=probs.device)
-        frac.index_add_(0, topi.reshape(-1), torch.ones(topi.numel(), dtype=torch.float32, device=probs.device))
-        frac = frac / topi.numel()
-        d_probs = d_probs + aux_scale * E * frac[None, :] / T
+        if balance is None:
+            balance = balance_loss_fwd(probs, topi)[2]
+        d_aux = aux_scale * balance.coef[None, :]
+        if mask is not None:
+            d_aux = torch.where(mask[:, None] != 0, d_aux, torch.zeros_like(d_aux))
+        d_probs = d_probs + d_aux
     return probs * (d_probs - (d_probs * probs).sum(-1, keepdim=True))
 
 
