@@ -113,6 +113,191 @@ def vocab_parallel_ce_bwd_(logits, labels, lse, grad_per_token, vocab_start: int
     return logits
 
 
+# ----------------------------------------------------------------------------- distillation from a teacher's top logits
+_TEACHER_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+MAX_TEACHER_ENTRIES = 1024
+
+
+def _distill_operands(what, logits, labels, top_ids, top_logits, temperature):
+    if logits.dim() != 2 or top_ids.dim() != 2 or top_ids.shape[0] != logits.shape[0] or top_logits.shape != top_ids.shape:
+        raise ValueError(f"{what}: logits [T, V], the teacher's ids and logits [T, K], got {tuple(logits.shape)}, {tuple(top_ids.shape)}, "
+                         f"{tuple(top_logits.shape)}")
+    if top_ids.dtype not in (torch.int32, torch.int64) or top_logits.dtype not in _TEACHER_TYPES or top_ids.shape[1] > MAX_TEACHER_ENTRIES:
+        raise ValueError(f"{what}: up to {MAX_TEACHER_ENTRIES} int32 or int64 ids with bf16, fp16 or fp32 logits a row, got "
+                         f"{top_ids.shape[1]} of {top_ids.dtype} and {top_logits.dtype}")
+    if labels is not None and (labels.shape != logits.shape[:1] or labels.dtype != torch.int32):
+        raise ValueError(f"{what}: {logits.shape[0]} int32 labels, got {labels.dtype} {tuple(labels.shape)}")
+    if not (0.0 < temperature < float("inf")):
+        raise ValueError(f"{what}: the temperature is positive and finite, not {temperature}")
+
+
+def _distill_native(what, logits, labels, top_ids, top_logits, *others):
+    """Operands as the kernels of csrc/distill.cu take them."""
+    if logits.dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError(f"{what}: the sm_100a kernel takes bf16 and fp32 logits, not {logits.dtype}")
+    if logits.stride(1) != 1 and logits.shape[1] > 1:
+        raise ValueError(f"{what}: the logits of a row lie side by side")
+    K.require_current_device(what, logits, labels, top_ids, top_logits, *others)
+    return (labels if labels is None or labels.is_contiguous() else labels.contiguous(),
+            top_ids if top_ids.stride(1) == 1 else top_ids.contiguous(),
+            top_logits if top_logits.stride(1) == 1 else top_logits.contiguous())
+
+
+_DISTILL_OPERANDS = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
+                     c_float]
+
+
+def _distill_arguments(logits, labels, ids, top, vocab_start, vocab, temperature):
+    T, Vl = logits.shape
+    return (logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), K.ptr(labels), ids.data_ptr(), ids.stride(0),
+            int(ids.dtype == torch.int64), top.data_ptr(), top.stride(0), _TEACHER_TYPES[top.dtype], T, Vl, ids.shape[1], vocab_start, vocab,
+            temperature)
+
+
+def _teacher_ref(top_ids, top_logits, vocab, temperature):
+    """``(q [T, K] fp32, log-sum-exp [T])``: the teacher's distribution over a row's entries (0 on padding) and its normaliser at the
+    temperature (+inf: the row has no entries)."""
+    t = torch.where((top_ids >= 0) & (top_ids < vocab), top_logits.float(), float("-inf")) / temperature
+    if not t.shape[1]:
+        return t, torch.full(t.shape[:1], float("inf"), device=t.device)
+    none = (t == float("-inf")).all(1)
+    lse = torch.where(none, float("inf"), torch.logsumexp(t, 1))
+    return torch.exp(t - lse[:, None]), lse
+
+
+def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature):
+    Vl = logits.shape[1]
+    lf = logits.float()
+    m = lf.max(dim=-1).values.clamp_min(torch.finfo(torch.float32).min)
+    rel = lf - m[:, None]
+    q, t_lse = _teacher_ref(top_ids, top_logits, vocab, temperature)
+    loc = top_ids.long() - vocab_start
+    own = (loc >= 0) & (loc < Vl) & (q != 0)
+    zero = torch.zeros_like(q)
+    dot = torch.where(own, q * rel.gather(1, loc.clamp(0, Vl - 1)), zero).sum(1)
+    ent = torch.where(q != 0, q * torch.log(torch.where(q != 0, q, 1.0)), zero).sum(1)
+    has = torch.zeros_like(m)
+    target = torch.zeros_like(m)
+    if labels is not None:
+        loc = labels.long() - vocab_start
+        inside = (labels >= 0) & (labels < vocab) & (loc >= 0) & (loc < Vl)
+        has = inside.float()
+        target = torch.where(inside, rel.gather(1, loc.clamp(0, Vl - 1)[:, None]).squeeze(1), target)
+    stats = torch.stack([m, torch.exp(rel).sum(1), torch.exp(rel / temperature).sum(1), target, dot, torch.where(own, q, zero).sum(1),
+                         torch.where(torch.isinf(t_lse) & (t_lse > 0), t_lse, ent), has], dim=1)
+    return stats, t_lse
+
+
+def _distill_combine_ref(all_stats, t_lse, temperature, hard):
+    m = all_stats[..., 0].max(dim=0).values
+    d = all_stats[..., 0] - m
+    lse = torch.log((all_stats[..., 1] * torch.exp(d)).sum(0))
+    lse_t = torch.log((all_stats[..., 2] * torch.exp(d / temperature)).sum(0))
+    seen = (all_stats[..., 1] != 0).any(0)                   # some logit of the row is not -inf
+    has, own = all_stats[..., 7] != 0, all_stats[..., 5]
+    target = torch.where(has, all_stats[..., 3] + d, 0.0).sum(0)
+    dot = torch.where(own != 0, all_stats[..., 4] + own * d, 0.0).sum(0)
+    ent = all_stats[0, :, 6]
+    is_hard, is_soft = has.any(0) & seen, (ent != float("inf")) & seen
+    ce = torch.where(is_hard, lse - target, 0.0) if hard else None
+    kd = torch.where(is_soft, temperature ** 2 * (ent - dot / temperature + lse_t), 0.0)
+    inf = torch.full_like(m, float("inf"))
+    return ce, kd, torch.stack([m, torch.where(is_hard, lse + m, inf), lse_t + m / temperature, torch.where(is_soft, t_lse, inf)], dim=1)
+
+
+def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature: float = 1.0, vocab_start: int = 0, group=None,
+                               sm_budget: int = 0, stream=None):
+    """Cross entropy and distillation loss per token, ``(ce [T], kd [T], saved [T, 4])`` in fp32.
+
+    ``logits [T, V/t]`` are the student's (bf16 or fp32), this rank's shard of the vocabulary from ``vocab_start`` on.  ``top_ids [T, K]``
+    and ``top_logits [T, K]`` are the ids and logits of the teacher's best entries, the same on every rank; an id outside the
+    vocabulary is padding.  With ``q = softmax(top_logits / temperature)`` over a row's entries and the student's ``p = softmax(logits /
+    temperature)`` over the whole vocabulary, ``kd = temperature^2 KL(q || p)``; rows without entries give 0.  ``ce`` is the cross entropy
+    against ``labels [T]`` int32 (0 where the label lies outside the vocabulary), or ``None`` without labels.  A row whose logits are
+    all ``-inf`` has neither loss nor gradient.  ``saved`` goes to
+    ``vocab_parallel_distill_bwd_``.  The ranks of ``group`` exchange eight numbers a token in one all-gather."""
+    if stream is not None:
+        return K.run_on_stream(stream, (logits, labels, top_ids, top_logits), lambda: vocab_parallel_distill_fwd(
+            logits, labels, top_ids, top_logits, temperature, vocab_start, group, sm_budget))
+    what = "vocab_parallel_distill_fwd"
+    _distill_operands(what, logits, labels, top_ids, top_logits, temperature)
+    T, Vl = logits.shape
+    ws = group_size(group)
+    vocab = Vl * ws
+    if not 0 <= vocab_start <= vocab - Vl:
+        raise ValueError(f"{what}: a shard of {Vl} entries from {vocab_start} on does not lie in a vocabulary of {vocab}")
+    native = K.use_native(logits)
+    if native:
+        labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits)
+        stats = torch.empty((T, 8), dtype=torch.float32, device=logits.device)
+        t_lse = torch.empty(T, dtype=torch.float32, device=logits.device)
+        fn = K.proto("dh_distill_stats", _DISTILL_OPERANDS + [c_void_p, c_void_p, c_int, c_void_p])
+        K.check(fn(*_distill_arguments(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature), stats.data_ptr(),
+                   t_lse.data_ptr(), sm_budget, K.stream_ptr()), "dh_distill_stats")
+    else:
+        stats, t_lse = _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature)
+    if ws > 1:
+        every = torch.empty((ws * T, 8), dtype=stats.dtype, device=stats.device)
+        dist.all_gather_into_tensor(every, stats, group=group)
+    else:
+        every = stats
+    if not native:
+        return _distill_combine_ref(every.view(ws, T, 8), t_lse, temperature, labels is not None)
+    ce = torch.empty(T, dtype=torch.float32, device=logits.device) if labels is not None else None
+    kd = torch.empty(T, dtype=torch.float32, device=logits.device)
+    saved = torch.empty((T, 4), dtype=torch.float32, device=logits.device)
+    fn = K.proto("dh_distill_combine", [c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
+    K.check(fn(every.data_ptr(), t_lse.data_ptr(), ws, T, temperature, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), K.stream_ptr()),
+            "dh_distill_combine")
+    return ce, kd, saved
+
+
+def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce, g_kd, temperature: float = 1.0, vocab_start: int = 0,
+                                out=None, sm_budget: int = 0, stream=None):
+    """Overwrites ``logits`` (or ``out``, of their shape and type) with ``d loss / d logits`` and returns it, for the gradients ``g_ce [T]``
+    and ``g_kd [T]`` (fp32) of what ``vocab_parallel_distill_fwd`` gave; the other arguments as there (``g_ce`` is ``None`` without
+    labels).  Rows with neither gradient become zero, whatever their logits."""
+    if stream is not None:
+        return K.run_on_stream(stream, (logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out), lambda: vocab_parallel_distill_bwd_(
+            logits, labels, top_ids, top_logits, saved, g_ce, g_kd, temperature, vocab_start, out, sm_budget))
+    what = "vocab_parallel_distill_bwd_"
+    _distill_operands(what, logits, labels, top_ids, top_logits, temperature)
+    T, Vl = logits.shape
+    out = logits if out is None else out
+    if out.shape != logits.shape or out.dtype != logits.dtype or (out.stride(0) < Vl and T > 1) or (out.stride(1) != 1 and Vl > 1):
+        raise ValueError(f"{what}: an output of the logits' shape and type with room for every row, got {out.dtype} {tuple(out.shape)}")
+    if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
+            and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+        raise ValueError(f"{what}: the output is the logits themselves or shares no memory with them")
+    if (g_ce is None) != (labels is None):
+        raise ValueError(f"{what}: labels and the gradient of their loss go together")
+    for t, shape in ((g_ce, (T,)), (g_kd, (T,)), (saved, (T, 4))):
+        if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous()):
+            raise ValueError(f"{what}: contiguous fp32 gradients [T] and saved statistics [T, 4], got {t.dtype} {tuple(t.shape)}")
+    if K.use_native(logits):
+        labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out)
+        fn = K.proto("dh_distill_grad", _DISTILL_OPERANDS + [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p])
+        K.check(fn(*_distill_arguments(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature), saved.data_ptr(),
+                   K.ptr(g_ce), g_kd.data_ptr(), out.data_ptr(), out.stride(0), sm_budget, K.stream_ptr()), "dh_distill_grad")
+        return out
+    lf = logits.float()
+    lse, lse_t, t_lse = saved[:, 1:2], saved[:, 2:3], saved[:, 3:4]
+    some = t_lse.squeeze(1) != float("inf")
+    gk = torch.where(some, g_kd, 0.0) * temperature
+    d = torch.where(gk[:, None] != 0, torch.exp(lf / temperature - lse_t) * gk[:, None], 0.0)
+    loc = top_ids.long() - vocab_start
+    own = (loc >= 0) & (loc < Vl) & (gk[:, None] != 0)
+    w = torch.where(own, torch.exp(top_logits.float() / temperature - t_lse) * gk[:, None], 0.0)
+    d.scatter_add_(1, loc.clamp(0, Vl - 1), -w)
+    if labels is not None:
+        loc = labels.long() - vocab_start
+        gc = torch.where(lse.squeeze(1) != float("inf"), g_ce, 0.0)
+        d = d + torch.where(gc[:, None] != 0, torch.exp(lf - lse) * gc[:, None], 0.0)
+        own = (loc >= 0) & (loc < Vl)
+        d.scatter_add_(1, loc.clamp(0, Vl - 1)[:, None], torch.where(own, -gc, 0.0)[:, None])
+    return out.copy_(d.to(out.dtype))
+
+
 def mask_scale_loss_fwd(loss_per_token, loss_mask, scale_func=None):
     """Masked mean with an optional loss-scaling hook (``optimizer.scale_loss`` in the
     reference: dhellam/operators/loss.py:131-164).  Returns ``(scaled_loss, sum, count)``."""

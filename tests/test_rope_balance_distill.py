@@ -1,0 +1,289 @@
+"""Rotary forms, balance loss and distillation on CPU: the reference path against 64 bits, refusals, ranks, gradients by differences."""
+import math
+
+import pytest
+import torch
+
+import operator_oracles as O
+from dhellam_b200.ops import loss as L
+from dhellam_b200.ops import moe as M
+from dhellam_b200.ops import rope as R
+
+
+# --------------------------------------------------------------------------- rotary
+def test_rope_frequencies_of_every_scaling():
+    """Against the definitions written per pair; the ends are exact: fast pairs stay, slow pairs are divided by the factor."""
+    r, theta, factor, old = 128, 500000.0, 8.0, 8192
+    plain, one = R.rope_frequencies(r, theta)
+    assert one == 1.0 and plain.dtype == torch.float64 and torch.allclose(plain, torch.tensor([theta ** (-2 * i / r) for i in range(r // 2)], dtype=torch.float64))
+    lin, _ = R.rope_frequencies(r, theta, R.RopeScaling("linear", factor, old))
+    assert torch.equal(lin, plain / factor)
+    ntk, _ = R.rope_frequencies(r, theta, R.RopeScaling("ntk", factor, old))
+    assert float(ntk[0]) == 1.0 and math.isclose(float(ntk[-1]), float(plain[-1]) / factor, rel_tol=1e-12)
+    llama, _ = R.rope_frequencies(r, theta, R.RopeScaling("llama3", factor, old))
+    for i in range(r // 2):
+        f, wave = float(plain[i]), 2 * math.pi / float(plain[i])
+        if wave < old / 4.0:
+            want = f
+        elif wave > old / 1.0:
+            want = f / factor
+        else:
+            smooth = (old / wave - 1.0) / (4.0 - 1.0)
+            want = (1 - smooth) * f / factor + smooth * f
+        assert math.isclose(float(llama[i]), want, rel_tol=1e-12), i
+    yarn, scale = R.rope_frequencies(r, theta, R.RopeScaling("yarn", factor, old))
+    assert math.isclose(scale, 0.1 * math.log(8.0) + 1.0)
+    ratio = yarn / plain
+    assert float(ratio[0]) == 1.0 and math.isclose(float(ratio[-1]), 1 / factor) and bool((ratio[1:] <= ratio[:-1] + 1e-15).all())
+    assert R.rope_frequencies(r, theta, R.RopeScaling("yarn", factor, old, attention_factor=1.25))[1] == 1.25
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("shape,r", [((7, 3, 16), 16), ((5, 2, 2, 10), 6), ((1, 1, 2), 2)])
+def test_rope_reference_and_its_backward(shape, r, interleaved):
+    torch.manual_seed(0)
+    q, k = torch.randn(*shape), torch.randn(*shape[:-2], 1, shape[-1])
+    pos = torch.randint(-5, 1000000, shape[:-2])
+    freq, _ = R.rope_frequencies(r, 10000.0)
+    q2, k2 = R.rope_fwd(q, k, pos, freq, interleaved, scale=1.2)
+    for x, y in ((q, q2), (k, k2)):
+        want, pair = O.rope(x, pos, freq, interleaved, 1.2)
+        assert bool(((y.double() - want).abs() <= O.rope_bound(want, pair, torch.float32)).all())
+        assert torch.equal(y[..., r:], x[..., r:])
+    # the backward is the transpose: <rope(x), y> = <x, rope_bwd(y)>, and by differences of a linear map
+    y = torch.randn(*shape)
+    back, _ = R.rope_bwd(y, None, pos, freq, interleaved, scale=1.2)
+    assert math.isclose(float((q2.double() * y.double()).sum()), float((q.double() * back.double()).sum()), rel_tol=1e-4, abs_tol=1e-4)
+    if not interleaved and r == shape[-1] and len(shape) == 3:
+        from dhellam_b200.ops.rope import rope_apply_, rope_table
+        pos = torch.arange(shape[0], dtype=torch.int32)
+        c, s = rope_table(16, r, 10000.0)
+        packed = torch.cat([q, k, k], 1).reshape(shape[0], -1)
+        rope_apply_(packed, pos, c, s, shape[1], 1, r)
+        q2, k2 = R.rope_fwd(q, k, pos, freq)
+        assert torch.allclose(packed[:, : shape[1] * r].view(q.shape), q2, atol=1e-6)
+
+
+def test_rope_in_place_and_refusals():
+    torch.manual_seed(1)
+    buf = torch.randn(6, 4, 8)
+    q, k = buf[:, :2], buf[:, 2:3]
+    pos, (freq, _) = torch.arange(6), R.rope_frequencies(8, 10000.0)
+    want = R.rope_fwd(q, k, pos, freq)
+    last = buf[:, 3].clone()
+    R.rope_fwd(q, k, pos, freq, out=(q, k))
+    assert torch.equal(q, want[0]) and torch.equal(k, want[1]) and torch.equal(buf[:, 3], last)
+    bad = [dict(positions=torch.arange(5)), dict(positions=pos.float()), dict(freq=freq.float()), dict(freq=torch.ones(5, dtype=torch.float64)),
+           dict(k=k[:, :, :6]), dict(k=k.double()), dict(q=buf.transpose(1, 2)), dict(out=(q[:5], k)), dict(out=(buf[:, 1:3], buf[:, 3:4])),
+           dict(out=(torch.empty(6, 1, 8).expand(6, 2, 8), torch.empty(6, 1, 8))), dict(out=(q, q[:, :1]))]
+    for b in bad:
+        args = dict(q=q, k=k, positions=pos, freq=freq) | b
+        with pytest.raises(ValueError):
+            R.rope_fwd(**args)
+    for b in (dict(kind="other"), dict(factor=0.5), dict(kind="llama3", factor=2.0, low_freq_factor=4.0), dict(original_max_position=0),
+              dict(kind="yarn", factor=2.0, beta_fast=1.0)):
+        with pytest.raises(ValueError):
+            R.RopeScaling(**b)
+    with pytest.raises(ValueError):
+        R.rope_frequencies(7, 10000.0)
+
+
+# --------------------------------------------------------------------------- balance
+def router_case(T, E, k, seed=0, device="cpu", masked=True):
+    g = torch.Generator().manual_seed(seed)
+    probs = torch.softmax(torch.randn(T, E, generator=g) * 2, -1)
+    top, ids = probs.topk(k, -1)
+    mask = torch.rand(T, generator=g) < 0.7 if masked else None
+    d = torch.randn(T, k, generator=g)
+    return [None if t is None else t.to(device) for t in (probs, ids, top / top.sum(-1, keepdim=True), d, mask)]
+
+
+@pytest.mark.parametrize("T,E,k,masked", [(0, 4, 2, False), (1, 1, 1, False), (37, 5, 2, True), (64, 8, 8, True), (9, 3, 1, False)])
+def test_balance_reference_against_64_bits(T, E, k, masked):
+    probs, ids, gates, dg, mask = router_case(T, E, k, masked=masked)
+    loss, counts, bal = M.balance_loss_fwd(probs, ids.to(torch.int32), mask)
+    want, wcounts, coef = O.balance(probs, ids, mask)
+    assert counts.dtype == torch.int32 and torch.equal(counts, wcounts)
+    assert abs(float(loss) - float(want)) <= O.EPS32 * (T + E + 20) * float(want)
+    if T and not masked:
+        assert torch.allclose(loss, M.aux_loss(probs, ids, E), rtol=1e-5)
+    got = M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=bal)
+    want, bound = O.router_gradient(dg, probs, ids, gates, 0.3, coef, mask)
+    assert bool(((got.double() - want).abs() <= bound).all())
+
+
+def test_router_gradient_by_differences():
+    """Of sum(d * gates(logits)) + w * balance(softmax(logits)) with the choices held, in 64 bits."""
+    T, E, k, w = 5, 6, 2, 0.7
+    probs, ids, gates, dg, mask = router_case(T, E, k, seed=3)
+    logits = probs.double().log()
+
+    def value(l):
+        p = torch.softmax(l, -1)
+        s = p.gather(1, ids)
+        return float((dg.double() * s / s.sum(-1, keepdim=True)).sum() + w * O.balance(p, ids, mask)[0])
+    got = M.router_topk_bwd(dg, probs, ids, gates, E, w, balance=M.balance_loss_fwd(probs, ids, mask)[2])
+    for t in range(T):
+        for e in range(E):
+            h = torch.zeros_like(logits)
+            h[t, e] = 1e-5
+            assert abs((value(logits + h) - value(logits - h)) / 2e-5 - float(got[t, e])) < 1e-5      # fp32 gradient, differences to 1e-9
+
+
+def test_balance_without_counted_tokens_and_with_choices_out_of_range():
+    probs, ids, gates, dg, _ = router_case(6, 4, 2)
+    loss, counts, bal = M.balance_loss_fwd(probs, ids, torch.zeros(6, dtype=torch.bool))
+    assert float(loss) == 0.0 and int(counts.sum()) == 0 and float(bal.coef.abs().sum()) == 0.0
+    ids[0] = torch.tensor([-1, 4])
+    ids[1, 1] = -1
+    loss, counts, bal = M.balance_loss_fwd(probs, ids)
+    assert int(counts.sum()) == 9
+    got = M.router_topk_bwd(dg, probs, ids, gates, 4, 0.3, balance=bal)
+    want, bound = O.router_gradient(dg, probs, ids, gates, 0.3, O.balance(probs, ids)[2])
+    assert bool(((got.double() - want).abs() <= bound).all())
+    probs = torch.full_like(probs, float("nan"))
+    mask = torch.ones(6, dtype=torch.uint8)
+    mask[2] = 0
+    clean = torch.softmax(torch.randn(6, 4), -1)
+    clean[2] = probs[2]
+    assert math.isfinite(float(M.balance_loss_fwd(clean, ids, mask)[0]))
+
+
+def test_balance_refusals():
+    probs, ids, gates, dg, mask = router_case(6, 4, 2)
+    bal = M.balance_loss_fwd(probs, ids)[2]
+    for bad in (lambda: M.balance_loss_fwd(probs.double(), ids), lambda: M.balance_loss_fwd(probs, ids.float()),
+                lambda: M.balance_loss_fwd(probs, ids[:5]), lambda: M.balance_loss_fwd(probs, ids, mask[:5]),
+                lambda: M.balance_loss_fwd(probs, ids, mask.float()), lambda: M.balance_loss_fwd(probs, ids[:, :0]),
+                lambda: M.router_topk_bwd(dg[:, :1], probs, ids, gates, 4), lambda: M.router_topk_bwd(dg, probs, ids, gates, 5),
+                lambda: M.router_topk_bwd(dg, probs, ids, gates[:5], 4),
+                lambda: M.router_topk_bwd(dg, probs, ids, gates, 4, 1.0, balance=M.Balance(bal.coef[:3], None))):
+        with pytest.raises(ValueError):
+            bad()
+
+
+# --------------------------------------------------------------------------- distillation
+def distill_case(T, V, K, seed=0, hard=True, dtype=torch.float32, teacher=torch.float32, scale=3.0):
+    """Rows with all entries, with padding, with none; a label twice among the teacher's ids; labels outside the vocabulary."""
+    g = torch.Generator().manual_seed(seed)
+    z = (torch.randn(T, V, generator=g) * scale).to(dtype)
+    ids = torch.randint(0, V, (T, K), generator=g, dtype=torch.int32)
+    top = (torch.randn(T, K, generator=g) * scale + 5).to(teacher)
+    labels = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    for t in range(T):
+        if t % 5 == 1 and K > 1:
+            ids[t, K // 2:] = torch.tensor([-1, V, V + 7])[t % 3]
+        if t % 7 == 2:
+            ids[t] = -1
+        if t % 4 == 3 and K > 1:
+            ids[t, 0] = ids[t, -1] = labels[t]
+        if t % 6 == 5:
+            labels[t] = (-100, V, V + 5)[t % 3]
+    g_ce, g_kd = torch.rand(T, generator=g), torch.rand(T, generator=g)
+    for t in range(T):
+        if t % 9 == 4:
+            g_ce[t] = g_kd[t] = 0.0
+    return z, labels if hard else None, ids, top, g_ce if hard else None, g_kd
+
+
+def check_distill(case, tau, ce, kd, grad, dtype):
+    z, labels, ids, top, g_ce, g_kd = case
+    want = O.distill(z, labels, ids.cpu(), top.cpu().double(), tau, g_ce, g_kd)
+    if labels is not None:
+        err = (ce.cpu().double() - want["ce"]).abs()
+        assert bool((err <= want["ce_bound"]).all()), float((err / want["ce_bound"].clamp_min(1e-30)).max())
+    err = (kd.cpu().double() - want["kd"]).abs()
+    assert bool((err <= want["kd_bound"]).all()), float((err / want["kd_bound"].clamp_min(1e-30)).max())
+    err = (grad.cpu().double() - want["grad"]).abs()
+    bound = want["grad_bound"] * (1 + O.HALF_STEP[dtype]) + O.HALF_STEP[dtype] * want["grad"].abs()
+    assert bool((err <= bound).all()), float((err / bound).max())
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.7, 3.3])
+@pytest.mark.parametrize("T,V,K,hard", [(20, 37, 5, True), (9, 64, 1, False), (1, 1, 1, True), (3, 11, 0, True), (0, 8, 2, True)])
+def test_distill_reference_against_64_bits(T, V, K, hard, tau):
+    case = z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, hard=hard)
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
+    assert (ce is None) == (not hard) and saved.shape == (T, 4)
+    out = torch.empty_like(z)
+    grad = L.vocab_parallel_distill_bwd_(z, labels, ids, top, saved, g_ce, g_kd, tau, out=out)
+    assert grad is out
+    check_distill(case, tau, ce, kd, grad, torch.float32)
+    keep = z.clone()
+    same = L.vocab_parallel_distill_bwd_(keep, labels, ids, top, saved, g_ce, g_kd, tau)
+    assert same is keep and torch.equal(keep, out)
+
+
+def test_distill_gradient_by_differences():
+    T, V, K, tau = 8, 9, 3, 1.7
+    z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, seed=5)
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
+    got = L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, tau)
+
+    def value(x):
+        r = O.distill(x, labels, ids, top.double(), tau)
+        return float((r["ce"] * g_ce.double()).sum() + (r["kd"] * g_kd.double()).sum())
+    for t in range(T):
+        for v in range(V):
+            h = torch.zeros(T, V, dtype=torch.float64)
+            h[t, v] = 1e-5
+            assert abs((value(z.double() + h) - value(z.double() - h)) / 2e-5 - float(got[t, v])) < 1e-5   # fp32 gradient, differences to 1e-9
+
+
+def test_distill_equals_cross_entropy_and_vanishes_for_the_students_own_distribution():
+    torch.manual_seed(2)
+    z, labels = torch.randn(6, 12), torch.randint(0, 12, (6,), dtype=torch.int32)
+    ids = torch.arange(12, dtype=torch.int64).expand(6, 12)
+    ce, kd, _ = L.vocab_parallel_distill_fwd(z, labels, ids, z.clone(), 2.0)
+    assert torch.allclose(ce, L.vocab_parallel_ce_fwd(z, labels)[0], atol=1e-5)
+    assert float(kd.abs().max()) < 1e-5
+
+
+def test_distill_masked_vocabulary_and_infinite_teacher():
+    """Entries of -inf in the student (a masked vocabulary) and in the teacher; a chosen entry of -inf costs infinitely much, one
+    without weight nothing."""
+    z = torch.randn(4, 10)
+    z[:, 7:] = float("-inf")
+    ids = torch.tensor([[0, 1, 8], [2, 3, 4], [8, 9, 7], [1, 2, 3]], dtype=torch.int32)
+    top = torch.tensor([[1.0, 2.0, float("-inf")], [1.0, 0.5, 0.0], [float("-inf")] * 3, [1.0, 2.0, 3.0]])
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, torch.tensor([0, 8, 1, 2], dtype=torch.int32), ids, top)
+    assert bool(torch.isfinite(kd).all()) and float(kd[2]) == 0.0 and float(ce[1]) == float("inf")
+    grad = L.vocab_parallel_distill_bwd_(z, torch.tensor([0, 8, 1, 2], dtype=torch.int32), ids, top, saved, torch.ones(4), torch.ones(4))
+    assert bool(torch.isfinite(grad).all()) and float(grad[3, 7:].abs().max()) == 0.0
+
+
+def test_distill_refusals():
+    z, labels, ids, top, g_ce, g_kd = distill_case(6, 9, 3)
+    saved = L.vocab_parallel_distill_fwd(z, labels, ids, top)[2]
+    fwd = dict(logits=z, labels=labels, top_ids=ids, top_logits=top)
+    for b in (dict(logits=z[0]), dict(labels=labels.long()), dict(labels=labels[:5]), dict(top_ids=ids.float()), dict(top_ids=ids[:5]),
+              dict(top_logits=top[:, :2]), dict(top_logits=top.double()), dict(temperature=0.0), dict(temperature=float("inf")),
+              dict(temperature=float("nan")), dict(temperature=-1.0), dict(vocab_start=1), dict(vocab_start=-1),
+              dict(top_ids=torch.zeros(6, 1025, dtype=torch.int32), top_logits=torch.zeros(6, 1025))):
+        with pytest.raises(ValueError):
+            L.vocab_parallel_distill_fwd(**(fwd | b))
+    wide = torch.zeros(6, 18)
+    bwd = fwd | dict(saved=saved, g_ce=g_ce, g_kd=g_kd)
+    for b in (dict(g_ce=None), dict(labels=None), dict(g_kd=g_kd.double()), dict(g_kd=g_kd[:5]), dict(saved=saved[:, :3]),
+              dict(out=torch.empty(6, 8)), dict(out=torch.empty(6, 9, dtype=torch.bfloat16)), dict(out=torch.empty(1, 9).expand(6, 9)),
+              dict(logits=wide[:, :9], out=wide[:, 9:]), dict(temperature=0.0)):
+        with pytest.raises(ValueError):
+            L.vocab_parallel_distill_bwd_(**(bwd | b))
+
+
+def _two_shards(rank, world):
+    z, labels, ids, top, g_ce, g_kd = distill_case(12, 24, 4, seed=9)
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, 1.6)
+    whole = L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, 1.6)
+    v0 = rank * 12
+    import torch.distributed as dist
+    shard = z[:, v0:v0 + 12].contiguous()
+    ce2, kd2, saved2 = L.vocab_parallel_distill_fwd(shard, labels, ids, top, 1.6, vocab_start=v0, group=dist.group.WORLD)
+    assert torch.allclose(ce, ce2, atol=1e-5) and torch.allclose(kd, kd2, atol=1e-5) and torch.allclose(saved, saved2, atol=1e-5)
+    grad = L.vocab_parallel_distill_bwd_(shard, labels, ids, top, saved2, g_ce, g_kd, 1.6, vocab_start=v0)
+    assert torch.allclose(grad, whole[:, v0:v0 + 12], atol=1e-6)
+
+
+def test_distill_over_two_vocabulary_shards():
+    from dist_utils import run_ranks
+    run_ranks(_two_shards, 2)
