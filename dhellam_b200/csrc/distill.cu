@@ -8,10 +8,16 @@
 // A label outside [0, V) gives ce = 0 and no gradient, a row without entries kd = 0 and none, a row whose logits are all -inf neither
 // loss nor gradient.  An id may stand twice; its weights add.
 //
-// Forward: one pass over the shard gives per row the maximum m, sum exp(z - m), sum exp((z - m) / tau), the label's and the chosen
-// entries' logits relative to m: eight numbers that the ranks exchange at once and one small kernel combines.  Sums are fp32.
-// Backward: one pass computes every element from (m, lse, lse at tau) and the few entries with a label or a teacher's weight are
+// Forward: one pass over the shard.  Every sum of exponentials is relative to a reference m that is a row's maximum or up to
+// D_RISE / log2 e below it: a thread takes the maximum of its first batch and moves it only when an element rises further, so the
+// rescaling leaves the loop and no term is below what its own rounding loses.  Exponentials are 2^((z - m) c) with c = log2 e or
+// log2 e / tau; the difference first, because (z - m) c is then right for the largest and the lowest finite logits too.  The teacher's sums
+// are linear in exp(t / tau), so one CTA needs two rounds of reductions in all.  Sums are fp32.
+// Backward: one pass computes every element from (m, 1 / sum, 1 / sum at tau) and the few entries with a label or a teacher's weight are
 // written once more behind it, from logits read before it, so that each element is rounded once.
+//
+// With both losses an element costs two exponentials, unless tau is 1 (they are the same) or 2 or 4 (exp(x) is a power of exp(x / tau):
+// one or two products).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -25,48 +31,123 @@
 
 namespace dh {
 
-constexpr int DT = 256;
+constexpr int DT = 256;                  // threads of a CTA
+constexpr int DW = DT / 32;
 constexpr int D_MAX_K = 1024;
+constexpr int D_BATCH = 4;               // 16-byte loads of a thread in flight
 constexpr float D_LOG2E = 1.4426950408889634f;
+constexpr float D_LN2 = 0.6931471805599453f;
+constexpr float D_RISE = 8.f;            // in powers of two; 2^-24 of it is what an exponent loses at most by a reference that is too low
 
+// Which exponentials an element needs: ONE (a single sum), TWO (both, on their own), SQUARE and FOURTH (tau = 2, 4).
+enum { D_ONE = 0, D_TWO = 1, D_SQUARE = 2, D_FOURTH = 3 };
+
+struct DistillArgs {
+  const void* z;                   // [T, Vl], row stride ld
+  const int* labels;               // nullable
+  const void* ids;                 // [T, K] int32 or int64
+  const void* t;                   // [T, K]
+  int64_t ld, id_stride, t_stride;
+  int id64, t_type;                // t_type: 0 bf16, 1 fp32, 2 fp16
+  int T, Vl, K, v0, V;
+  float tau, inv_tau;
+};
+
+__device__ __forceinline__ float d_ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float d_max(float a, float b) { return (a > b || a != a) ? a : b; }      // a NaN stays
 __device__ __forceinline__ float d_warp_sum(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-__device__ __forceinline__ float d_max(float a, float b) { return (a > b || a != a) ? a : b; }      // a NaN stays
 __device__ __forceinline__ float d_warp_max(float v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = d_max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// Over the CTA; every thread gets the result.  `red`: 32 floats, free again behind the next barrier.
-__device__ __forceinline__ float d_block_sum(float v, float* red) {
-  v = d_warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return d_warp_sum((threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : 0.f);
+
+// Two fp32 in one register pair: the packed forms of add, multiply and fma need one issue slot for two elements.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+  return r;
 }
-__device__ __forceinline__ float d_block_max(float v, float* red) {
-  v = d_warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return d_warp_max((threadIdx.x & 31) < (blockDim.x >> 5) ? red[threadIdx.x & 31] : -INFINITY);
+__device__ __forceinline__ float2 f2_get(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator+(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 operator*(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_ex2(F2 a) {
+  const float2 x = f2_get(a);
+  return f2(d_ex2(x.x), d_ex2(x.y));
 }
 
-struct DistillArgs {
-  const void* z;                   // [T, Vl], row stride ld
-  long long ld;
-  const int* labels;               // nullable
-  const void* ids;                 // [T, K] int32 or int64
-  long long id_stride;
-  const void* t;                   // [T, K]
-  long long t_stride;
-  int id64, t_type;                // t_type: 0 bf16, 1 fp32, 2 fp16
-  int T, Vl, K, v0, V;
-  float inv_tau;
+// 16 bytes of logits as pairs of fp32, and their largest.
+template <typename T> struct DVec;
+template <> struct DVec<__nv_bfloat16> {
+  static constexpr int N = 8;
+  __device__ static __forceinline__ void unpack(const uint4& u, F2 (&x)[4]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+  }
+  __device__ static __forceinline__ uint4 pack(const F2 (&x)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const float2 f = f2_get(x[i]); w[i] = pack_bf16x2(f.x, f.y); }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __device__ static __forceinline__ float largest(const uint4 (&u)[D_BATCH]) {
+    __nv_bfloat162 m = __hmax2(as2(u[0].x), as2(u[0].y));
+    m = __hmax2(m, __hmax2(as2(u[0].z), as2(u[0].w)));
+#pragma unroll
+    for (int i = 1; i < D_BATCH; ++i) {
+      m = __hmax2(m, __hmax2(as2(u[i].x), as2(u[i].y)));
+      m = __hmax2(m, __hmax2(as2(u[i].z), as2(u[i].w)));
+    }
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  __device__ static __forceinline__ __nv_bfloat162 as2(uint32_t u) { return *reinterpret_cast<__nv_bfloat162*>(&u); }
+};
+template <> struct DVec<float> {
+  static constexpr int N = 4;
+  __device__ static __forceinline__ void unpack(const uint4& u, F2 (&x)[2]) {
+    x[0] = f2(__uint_as_float(u.x), __uint_as_float(u.y));
+    x[1] = f2(__uint_as_float(u.z), __uint_as_float(u.w));
+  }
+  __device__ static __forceinline__ uint4 pack(const F2 (&x)[2]) {
+    const float2 a = f2_get(x[0]), b = f2_get(x[1]);
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+  }
+  __device__ static __forceinline__ float largest(const uint4 (&u)[D_BATCH]) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < D_BATCH; ++i)
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(u[i].x), __uint_as_float(u[i].y)), fmaxf(__uint_as_float(u[i].z), __uint_as_float(u[i].w))));
+    return m;
+  }
 };
 
 __device__ __forceinline__ float d_load(const float* p) { return *p; }
@@ -74,180 +155,416 @@ __device__ __forceinline__ float d_load(const __nv_bfloat16* p) { return __bfloa
 __device__ __forceinline__ void d_store(float* p, float v) { *p = v; }
 __device__ __forceinline__ void d_store(__nv_bfloat16* p, float v) { *p = __float2bfloat16(v); }
 
-__device__ __forceinline__ float d_teacher(const DistillArgs& a, long long row, int j) {
-  const long long i = row * a.t_stride + j;
+__device__ __forceinline__ float d_teacher(const DistillArgs& a, int64_t row, int j) {
+  const int64_t i = row * a.t_stride + j;
   if (a.t_type == 1) return reinterpret_cast<const float*>(a.t)[i];
   if (a.t_type == 0) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(a.t)[i]);
   return __half2float(reinterpret_cast<const __half*>(a.t)[i]);
 }
 // The vocabulary entry of the teacher's j-th logit, -1 for padding.
-__device__ __forceinline__ int d_id(const DistillArgs& a, long long row, int j) {
-  const long long i = row * a.id_stride + j;
-  const long long v = a.id64 ? reinterpret_cast<const long long*>(a.ids)[i] : (long long)reinterpret_cast<const int*>(a.ids)[i];
+__device__ __forceinline__ int d_id(const DistillArgs& a, int64_t row, int j) {
+  const int64_t i = row * a.id_stride + j;
+  const int64_t v = a.id64 ? reinterpret_cast<const int64_t*>(a.ids)[i] : (int64_t)reinterpret_cast<const int*>(a.ids)[i];
   return v < 0 || v >= a.V ? -1 : (int)v;
 }
 
-// Eight numbers per row: m, sum exp(z - m), sum exp((z - m) / tau), z_label - m (0: not in this shard), sum q (z_id - m) and sum q over
-// the entries in this shard, sum q log q (+inf: the row has no entries), 1 if the label is in this shard.
+// A row's elements in 16-byte vectors of the memory they lie in: `lead` elements before the first, then `vecs`, the rest behind them.
+// Part p of n: vectors [v0, v1), the lead with the first part, the rest with the last.
+struct DSpan {
+  int lead, vecs, v0, v1, c0, c1;        // c0, c1: this part's elements
+};
 template <typename T>
-__global__ void __launch_bounds__(DT) distill_stats_kernel(const DistillArgs a, float* __restrict__ stats, float* __restrict__ teacher_lse) {
-  __shared__ float red[32];
-  for (int row = blockIdx.x; row < a.T; row += gridDim.x) {
-    const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
-    float m = -FLT_MAX, s = 0.f, st = 0.f;
-    for (int c = threadIdx.x; c < a.Vl; c += DT) {
-      const float v = d_load(z + c);
-      if (v > m) {
-        s *= exp2f((m - v) * D_LOG2E);
-        st *= exp2f((m - v) * D_LOG2E * a.inv_tau);
-        m = v;
-      }
-      const float x = (v - m) * D_LOG2E;
-      s += exp2f(x);
-      st += exp2f(x * a.inv_tau);
+__device__ __forceinline__ DSpan d_span(const T* row, int n, int part, int parts) {
+  constexpr int N = DVec<T>::N;
+  DSpan s;
+  s.lead = min(n, (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T));
+  s.vecs = (n - s.lead) / N;
+  s.v0 = (int)((int64_t)s.vecs * part / parts);
+  s.v1 = (int)((int64_t)s.vecs * (part + 1) / parts);
+  s.c0 = part == 0 ? 0 : s.lead + s.v0 * N;
+  s.c1 = part == parts - 1 ? n : s.lead + s.v1 * N;
+  return s;
+}
+
+// Sums of one thread relative to its reference.
+template <int MODE>
+struct DSums {
+  float m = -FLT_MAX;
+  F2 s1 = f2(0.f, 0.f), st = f2(0.f, 0.f);         // ONE: st alone
+  __device__ __forceinline__ void raise(float to, float c1, float ct) {
+    const float f = d_ex2((m - to) * ct);
+    st = st * f2(f, f);
+    if (MODE != D_ONE) {
+      const float g = d_ex2((m - to) * c1);
+      s1 = s1 * f2(g, g);
     }
-    const float gm = d_block_max(m, red);
-    s = d_block_sum(s * exp2f((m - gm) * D_LOG2E), red);
-    st = d_block_sum(st * exp2f((m - gm) * D_LOG2E * a.inv_tau), red);
-    // the teacher's distribution over the row's entries
+    m = to;
+  }
+  __device__ __forceinline__ void add(F2 z, F2 nm, F2 c1, F2 ct) {
+    const F2 x = z + nm;
+    const F2 e = f2_ex2(x * ct);
+    st = st + e;
+    if (MODE == D_TWO) s1 = s1 + f2_ex2(x * c1);
+    if (MODE == D_SQUARE) s1 = f2_fma(e, e, s1);
+    if (MODE == D_FOURTH) { const F2 q = e * e; s1 = f2_fma(q, q, s1); }
+  }
+};
+
+// What a row's sums give.  m: reference; s1, st: sums; target: (z_label - m) log2 e (+inf: no label here); dot, own: sums of q (z_id - m)
+// log2 e / tau and of q over the entries here; ent: sum of q log q (+inf: the row has no entries); tl: the teacher's lse at tau.
+__device__ __forceinline__ void d_finish(float m, float s1, float st, float target, float dot, float ent, float tl, float tau, float* ce,
+                                         float* kd, float4* saved) {
+  const bool hard = target != INFINITY && s1 != 0.f, soft = ent != INFINITY && st != 0.f;      // a sum of 0: all logits are -inf
+  if (ce != nullptr) *ce = hard ? D_LN2 * (log2f(s1) - target) : 0.f;
+  *kd = soft ? tau * tau * (ent + D_LN2 * (log2f(st) - dot)) : 0.f;
+  *saved = make_float4(m, hard ? 1.f / s1 : 0.f, soft ? 1.f / st : 0.f, soft ? tl : INFINITY);
+}
+
+// One cluster of CTAs per row (one CTA where there are rows enough); they share its vectors and the first one joins their sums.
+// Where `stats` is given (the vocabulary is divided among ranks) a row's eight numbers go there: m, s1, st, target, dot, own, ent, tl.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a, int parts, float* __restrict__ ce, float* __restrict__ kd,
+                                                            float4* __restrict__ saved, float4* __restrict__ stats) {
+  constexpr int N = DVec<T>::N;
+  __shared__ float red[2][DW];
+  __shared__ float sums[DW][6];
+  __shared__ float join[4];                          // this CTA's m, s1, st for the first one of its cluster
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int part = blockIdx.x % parts;
+  const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
+  const float cr = MODE == D_ONE ? ct : fmaxf(c1, ct);
+  const F2 c1p = f2(c1, c1), ctp = f2(ct, ct);
+  for (int row = blockIdx.x / parts; row < a.T; row += gridDim.x / parts) {
+    const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
+    const DSpan sp = d_span(z, a.Vl, part, parts);
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
+    DSums<MODE> acc;
+    F2 x[N / 2];
+    int i = sp.v0 + threadIdx.x;
+    for (; i + (D_BATCH - 1) * DT < sp.v1; i += D_BATCH * DT) {
+      uint4 u[D_BATCH];
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b) u[b] = ld_nc_v4(zv + i + b * DT);
+      const float lm = DVec<T>::largest(u);
+      if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
+      const F2 nm = f2(-acc.m, -acc.m);
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b) {
+        DVec<T>::unpack(u[b], x);
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) acc.add(x[j], nm, c1p, ctp);
+      }
+    }
+    for (; i < sp.v1; i += DT) {
+      uint4 u[D_BATCH];
+      u[0] = ld_nc_v4(zv + i);
+#pragma unroll
+      for (int b = 1; b < D_BATCH; ++b) u[b] = u[0];
+      const float lm = DVec<T>::largest(u);
+      if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
+      const F2 nm = f2(-acc.m, -acc.m);
+      DVec<T>::unpack(u[0], x);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) acc.add(x[j], nm, c1p, ctp);
+    }
+    float s1, st;
+    {
+      const float2 p = f2_get(acc.s1), q = f2_get(acc.st);
+      s1 = p.x + p.y;
+      st = q.x + q.y;
+    }
+    // elements before the first and behind the last vector
+    auto single = [&](int c) {
+      const float v = d_load(z + c);
+      if ((v - acc.m) * cr > D_RISE) {
+        s1 *= d_ex2((acc.m - v) * c1);
+        st *= d_ex2((acc.m - v) * ct);
+        acc.m = v;
+      }
+      st += d_ex2((v - acc.m) * ct);
+      if (MODE != D_ONE) s1 += d_ex2((v - acc.m) * c1);
+    };
+    if (part == 0 && (int)threadIdx.x < sp.lead) single(threadIdx.x);
+    if (part == parts - 1 && sp.lead + sp.vecs * N + (int)threadIdx.x < a.Vl) single(sp.lead + sp.vecs * N + threadIdx.x);
+    // first round: the CTA's reference and the teacher's largest logit
     float tm = -INFINITY;
-    for (int j = threadIdx.x; j < a.K; j += DT)
-      if (d_id(a, row, j) >= 0) tm = d_max(tm, d_teacher(a, row, j));
-    tm = d_block_max(tm, red);
-    const bool some = tm != -INFINITY;
-    float w = 0.f;
-    if (some)
+    if (part == 0)
       for (int j = threadIdx.x; j < a.K; j += DT)
-        if (d_id(a, row, j) >= 0) w += expf((d_teacher(a, row, j) - tm) * a.inv_tau);
-    w = d_block_sum(w, red);
-    const float lw = logf(w);
-    float dot = 0.f, own = 0.f, ent = 0.f;
-    if (some)
+        if (d_id(a, row, j) >= 0) tm = d_max(tm, d_teacher(a, row, j));
+    const float wm = d_warp_max(acc.m);
+    tm = d_warp_max(tm);
+    if (lane == 0) { red[0][w] = wm; red[1][w] = tm; }
+    __syncthreads();
+    float m = red[0][0];
+    tm = red[1][0];
+#pragma unroll
+    for (int q = 1; q < DW; ++q) { m = d_max(m, red[0][q]); tm = d_max(tm, red[1][q]); }
+    // second round: the sums; the teacher's relative to its largest
+    float v[6] = {s1 * d_ex2((acc.m - m) * c1), st * d_ex2((acc.m - m) * ct), 0.f, 0.f, 0.f, 0.f};
+    if (part == 0 && tm != -INFINITY)
       for (int j = threadIdx.x; j < a.K; j += DT) {
         const int id = d_id(a, row, j);
         if (id < 0) continue;
-        const float lq = (d_teacher(a, row, j) - tm) * a.inv_tau - lw;
-        const float q = expf(lq);
+        const float lt = (d_teacher(a, row, j) - tm) * a.inv_tau;
+        const float q = expf(lt);
         if (q == 0.f) continue;                          // no weight: its logit may be infinite
-        ent += q * lq;
+        v[2] += q;
+        v[3] += q * lt;
         const int loc = id - a.v0;
         if (loc >= 0 && loc < a.Vl) {
-          dot += q * (d_load(z + loc) - gm);
-          own += q;
+          v[4] += q * ((d_load(z + loc) - m) * ct);
+          v[5] += q;
         }
       }
-    dot = d_block_sum(dot, red);
-    own = d_block_sum(own, red);
-    ent = d_block_sum(ent, red);
-    if (threadIdx.x == 0) {
+#pragma unroll
+    for (int q = 0; q < 6; ++q) v[q] = d_warp_sum(v[q]);
+    if (lane == 0) {
+#pragma unroll
+      for (int q = 0; q < 6; ++q) sums[w][q] = v[q];
+    }
+    __syncthreads();
+    if (w == 0) {
+      float t = 0.f;
+      if (lane < 6) {
+#pragma unroll
+        for (int q = 0; q < DW; ++q) t += sums[q][lane];
+      }
+#pragma unroll
+      for (int q = 0; q < 6; ++q) v[q] = __shfl_sync(0xffffffffu, t, q);
+      if (lane == 0 && parts > 1) { join[0] = m; join[1] = v[0]; join[2] = v[1]; }
+    }
+    __syncwarp();
+    if (parts > 1) cluster_sync_all();
+    if (part == 0 && threadIdx.x == 0) {
+      float dot = v[4], own = v[5];
       const int lab = a.labels != nullptr ? a.labels[row] : -1;
       const int loc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
-      const bool in = loc >= 0 && loc < a.Vl;
-      float4* o = reinterpret_cast<float4*>(stats + (size_t)row * 8);
-      o[0] = make_float4(gm, s, st, in ? d_load(z + loc) - gm : 0.f);
-      o[1] = make_float4(dot, own, some ? ent : INFINITY, in ? 1.f : 0.f);
-      teacher_lse[row] = some ? tm * a.inv_tau + lw : INFINITY;
+      float target = loc >= 0 && loc < a.Vl ? (d_load(z + loc) - m) * c1 : INFINITY;
+      for (int r = 1; r < parts; ++r) {
+        const uint32_t at = mapa_u32(smem_u32(join), r);
+        const float om = __uint_as_float(ld_cluster_u32(at)), o1 = __uint_as_float(ld_cluster_u32(at + 4)),
+                    ot = __uint_as_float(ld_cluster_u32(at + 8));
+        const float to = d_max(m, om);
+        v[0] = v[0] * d_ex2((m - to) * c1) + o1 * d_ex2((om - to) * c1);
+        v[1] = v[1] * d_ex2((m - to) * ct) + ot * d_ex2((om - to) * ct);
+        if (own != 0.f) dot += own * ((m - to) * ct);
+        target += (m - to) * c1;
+        m = to;
+      }
+      if (MODE == D_ONE) v[0] = v[1];
+      const float ent = tm != -INFINITY ? v[3] / v[2] - logf(v[2]) : INFINITY;
+      const float tl = tm != -INFINITY ? tm * a.inv_tau + logf(v[2]) : INFINITY;
+      if (own != 0.f) { dot /= v[2]; own /= v[2]; }
+      if (stats != nullptr) {
+        stats[(size_t)row * 2] = make_float4(m, v[0], v[1], target);
+        stats[(size_t)row * 2 + 1] = make_float4(dot, own, ent, tl);
+      } else {
+        d_finish(m, v[0], v[1], target, dot, ent, tl, a.tau, ce != nullptr ? ce + row : nullptr, kd + row, saved + row);
+      }
     }
+    __syncwarp();
+    if (parts > 1) cluster_sync_all();               // nobody leaves or writes anew while the first CTA reads
   }
 }
 
-// stats [R, T, 8] of the ranks -> ce [T] (nullable), kd [T], saved [T, 4] = (m, lse(z) or +inf where ce has no gradient, lse(z / tau),
-// the teacher's lse at tau or +inf where kd has none).
-__global__ void __launch_bounds__(DT) distill_combine_kernel(const float4* __restrict__ stats, const float* __restrict__ teacher_lse, int R, int T,
-                                                             float tau, float* __restrict__ ce, float* __restrict__ kd, float4* __restrict__ saved) {
+// stats [R, T, 8] of the ranks -> ce [T] (nullable), kd [T], saved [T, 4] = (m, 1 / sum or 0 where ce has no gradient, 1 / sum at tau,
+// the teacher's lse at tau or +inf where kd has no gradient).
+__global__ void __launch_bounds__(DT) distill_combine_kernel(const float4* __restrict__ stats, int R, int T, float tau, float* __restrict__ ce,
+                                                             float* __restrict__ kd, float4* __restrict__ saved) {
   const int t = blockIdx.x * DT + threadIdx.x;
   if (t >= T) return;
+  const float ct = D_LOG2E / tau;
   float m = stats[(size_t)t * 2].x;
   for (int r = 1; r < R; ++r) m = d_max(m, stats[((size_t)r * T + t) * 2].x);
-  const float it = 1.f / tau;
-  float s = 0.f, st = 0.f, target = 0.f, has = 0.f, dot = 0.f, ent = 0.f;
+  float s1 = 0.f, st = 0.f, target = INFINITY, dot = 0.f, ent = 0.f, tl = 0.f;
   for (int r = 0; r < R; ++r) {
     const float4 u = stats[((size_t)r * T + t) * 2], v = stats[((size_t)r * T + t) * 2 + 1];
     const float d = u.x - m;
-    s += u.y * expf(d);
-    st += u.z * expf(d * it);
-    if (v.w != 0.f) { target += u.w + d; has = 1.f; }
-    if (v.y != 0.f) dot += v.x + v.y * d;
+    s1 += u.y * d_ex2(d * D_LOG2E);
+    st += u.z * d_ex2(d * ct);
+    if (u.w != INFINITY) target = u.w + d * D_LOG2E;
+    if (v.y != 0.f) dot += v.x + v.y * (d * ct);
     ent = v.z;
+    tl = v.w;
   }
-  const float l = logf(s), lt = logf(st);
-  const bool hard = has != 0.f && s != 0.f, soft = ent != INFINITY && s != 0.f;      // s = 0: all logits are -inf
-  if (ce != nullptr) ce[t] = hard ? l - target : 0.f;
-  kd[t] = soft ? tau * tau * (ent - dot * it + lt) : 0.f;
-  saved[t] = make_float4(m, hard ? l + m : INFINITY, lt + m * it, soft ? teacher_lse[t] : INFINITY);
+  d_finish(m, s1, st, target, dot, ent, tl, tau, ce != nullptr ? ce + t : nullptr, kd + t, saved + t);
 }
 
-// out = d loss / d z; out may be z.  One CTA per row.
-template <typename T>
-__global__ void __launch_bounds__(DT) distill_grad_kernel(const DistillArgs a, const float4* __restrict__ saved, const float* __restrict__ g_ce,
-                                                          const float* __restrict__ g_kd, float tau, void* out, long long out_ld) {
-  __shared__ int ids[D_MAX_K + 1];          // entries of this shard that get more than the softmax: the teacher's, then the label
+// out = d loss / d z; out may be z.  One CTA per part of a row.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(DT, 4) distill_bwd_kernel(const DistillArgs a, int parts, const float4* __restrict__ saved,
+                                                            const float* __restrict__ g_ce, const float* __restrict__ g_kd, void* out,
+                                                            int64_t out_ld) {
+  constexpr int N = DVec<T>::N;
+  __shared__ int ids[D_MAX_K + 1];          // entries of this part that get more than the softmax: the teacher's, then the label
   __shared__ float add[D_MAX_K + 1], at[D_MAX_K + 1];
-  for (int row = blockIdx.x; row < a.T; row += gridDim.x) {
+  const int part = blockIdx.x % parts;
+  const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
+  for (int row = blockIdx.x / parts; row < a.T; row += gridDim.x / parts) {
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
     T* o = reinterpret_cast<T*>(out) + row * out_ld;
+    const DSpan sp = d_span(z, a.Vl, part, parts);
     const float4 sv = saved[row];
-    const bool some = sv.w != INFINITY;
-    const int lab = a.labels != nullptr ? a.labels[row] : -1;
-    const bool hard = a.labels != nullptr && sv.y != INFINITY;
-    const float gc = hard ? g_ce[row] : 0.f, gk = some ? g_kd[row] * tau : 0.f;
+    const float gc = a.labels != nullptr && sv.y != 0.f ? g_ce[row] : 0.f, gk = sv.w != INFINITY ? g_kd[row] * a.tau : 0.f;
+    const float A = gc != 0.f ? gc * sv.y : 0.f, B = gk != 0.f ? gk * sv.z : 0.f;
     __syncthreads();
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       int loc = -1;
-      float w = 0.f;
+      float g = 0.f;
       if (j == a.K) {
-        if (hard) { loc = lab - a.v0; w = gc; }
+        if (gc != 0.f) { loc = a.labels[row] - a.v0; g = gc; }
       } else if (gk != 0.f) {
         const int id = d_id(a, row, j);
-        if (id >= 0) { loc = id - a.v0; w = gk * expf(d_teacher(a, row, j) * a.inv_tau - sv.w); }
+        if (id >= 0) { loc = id - a.v0; g = gk * expf(d_teacher(a, row, j) * a.inv_tau - sv.w); }
       }
-      const bool in = loc >= 0 && loc < a.Vl;
+      const bool in = loc >= sp.c0 && loc < sp.c1;
       ids[j] = in ? loc : -1;
-      add[j] = w;
+      add[j] = g;
       at[j] = in ? d_load(z + loc) : 0.f;
     }
     __syncthreads();
-    if (gc == 0.f && gk == 0.f) {             // a token without loss: zeros, whatever its logits
-      for (int c = threadIdx.x; c < a.Vl; c += DT) d_store(o + c, 0.f);
-      continue;
-    }
-    auto soft = [&](float v) {
-      float g = 0.f;
-      if (gc != 0.f) g += gc * expf(v - sv.y);
-      if (gk != 0.f) g += gk * expf(v * a.inv_tau - sv.z);
-      return g;
+    const bool zero = gc == 0.f && gk == 0.f;        // a token without loss: zeros, whatever its logits
+    const F2 nm = f2(-sv.x, -sv.x), c1p = f2(c1, c1), ctp = f2(ct, ct), Ap = f2(A, A), Bp = f2(B, B);
+    auto soft2 = [&](F2 v) {
+      const F2 x = v + nm;
+      const F2 e = f2_ex2(x * ctp);
+      if (MODE == D_ONE) return e * (Ap + Bp);
+      if (MODE == D_TWO) return f2_fma(f2_ex2(x * c1p), Ap, e * Bp);
+      const F2 q = e * e;
+      return f2_fma(MODE == D_SQUARE ? q : q * q, Ap, e * Bp);
     };
-    for (int c = threadIdx.x; c < a.Vl; c += DT) d_store(o + c, soft(d_load(z + c)));
+    auto soft = [&](float v) { return f2_get(soft2(f2(v, v))).x; };
+    auto single = [&](int c) { d_store(o + c, zero ? 0.f : soft(d_load(z + c))); };
+    if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(o)) & 15) != 0) {
+      for (int c = sp.c0 + threadIdx.x; c < sp.c1; c += DT) single(c);      // rows that are aligned differently
+    } else {
+      const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
+      uint4* ov = reinterpret_cast<uint4*>(o + sp.lead);
+      if (part == 0 && (int)threadIdx.x < sp.lead) single(threadIdx.x);
+      if (part == parts - 1 && sp.lead + sp.vecs * N + (int)threadIdx.x < a.Vl) single(sp.lead + sp.vecs * N + threadIdx.x);
+      if (zero) {
+        for (int i = sp.v0 + threadIdx.x; i < sp.v1; i += DT) ov[i] = make_uint4(0, 0, 0, 0);
+      } else {
+        auto vec = [&](const uint4& u) {
+          F2 x[N / 2];
+          DVec<T>::unpack(u, x);
+#pragma unroll
+          for (int j = 0; j < N / 2; ++j) x[j] = soft2(x[j]);
+          return DVec<T>::pack(x);
+        };
+        int i = sp.v0 + threadIdx.x;
+        for (; i + (D_BATCH - 1) * DT < sp.v1; i += D_BATCH * DT) {
+          uint4 u[D_BATCH];
+#pragma unroll
+          for (int b = 0; b < D_BATCH; ++b) u[b] = zv[i + b * DT];
+#pragma unroll
+          for (int b = 0; b < D_BATCH; ++b) ov[i + b * DT] = vec(u[b]);
+        }
+        for (; i < sp.v1; i += DT) ov[i] = vec(zv[i]);
+      }
+    }
     __syncthreads();
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       const int id = ids[j];
-      if (id < 0) continue;
+      if (id < 0 || zero) continue;
       bool first = true;
-      float w = add[j];
+      float g = add[j];
       for (int i = 0; i <= a.K; ++i) {
         if (i == j || ids[i] != id) continue;
         if (i < j) first = false;
-        else w += add[i];
+        else g += add[i];
       }
-      if (first) d_store(o + id, soft(at[j]) - w);
+      if (first) d_store(o + id, soft(at[j]) - g);
     }
   }
 }
 
-static int d_refuse(const char* what, int T, int Vl, int K, int v0, int V, float inv_tau) {
-  if (T >= 0 && Vl > 0 && K >= 0 && K <= D_MAX_K && v0 >= 0 && V >= v0 + (int64_t)Vl && inv_tau > 0.f && inv_tau <= FLT_MAX) return 0;
-  set_last_error_c(what, "a shard inside the vocabulary, at most 1024 teacher's entries, a positive temperature");
+// ---------------------------------------------------------------------------- host
+// All fields 8 bytes wide, as the Python layer packs them.
+struct DistillCall {
+  int64_t z, ld, f32, labels, ids, id_stride, id64, t, t_stride, t_type, T, Vl, K, v0, V, budget, stream;
+  double tau;
+};
+
+static int d_refuse(const char* what, const DistillCall& c) {
+  if (c.T >= 0 && c.T <= INT32_MAX && c.Vl > 0 && c.K >= 0 && c.K <= D_MAX_K && c.v0 >= 0 && c.V >= c.v0 + c.Vl && c.V <= INT32_MAX &&
+      c.tau > 0. && 1. / c.tau <= FLT_MAX && (float)c.tau > 0.f && (float)c.tau <= FLT_MAX)
+    return 0;
+  set_last_error_c(what, "a shard inside a vocabulary of at most 2^31 - 1 entries, at most 1024 teacher's entries, a positive temperature");
   return (int)cudaErrorInvalidValue;
 }
-static int d_rc(const char* what) {
-  cudaError_t e = cudaGetLastError();
+static int d_rc(const char* what, cudaError_t e) {
+  if (e == cudaSuccess) e = cudaGetLastError();
   if (e != cudaSuccess) set_last_error_c(what, cudaGetErrorString(e));
   return (int)e;
 }
-static int d_grid(int64_t rows, int sm_budget) {
+static DistillArgs d_args(const DistillCall& c) {
+  DistillArgs a;
+  a.z = (const void*)c.z;
+  a.labels = (const int*)c.labels;
+  a.ids = (const void*)c.ids;
+  a.t = (const void*)c.t;
+  a.ld = c.ld;
+  a.id_stride = c.id_stride;
+  a.t_stride = c.t_stride;
+  a.id64 = (int)c.id64;
+  a.t_type = (int)c.t_type;
+  a.T = (int)c.T;
+  a.Vl = (int)c.Vl;
+  a.K = (int)c.K;
+  a.v0 = (int)c.v0;
+  a.V = (int)c.V;
+  a.tau = (float)c.tau;
+  a.inv_tau = (float)(1. / c.tau);
+  return a;
+}
+static int d_mode(const DistillCall& c) {
+  if (c.labels == 0 || c.tau == 1.) return D_ONE;
+  return c.tau == 2. ? D_SQUARE : c.tau == 4. ? D_FOURTH : D_TWO;
+}
+// CTAs that share a row: where there are fewer rows than the GPU holds CTAs, as long as each thread still has a vector.
+static int d_parts(const DistillCall& c, int per_vec, int most) {
   const int sms = dh_sm_count();
-  const int budget = (sm_budget <= 0 || sm_budget > sms) ? sms : sm_budget;
-  return (int)(rows < (int64_t)budget * 8 ? rows : (int64_t)budget * 8);
+  const int64_t room = 4ll * ((c.budget <= 0 || c.budget > sms) ? sms : c.budget);
+  int parts = 1;
+  while (parts < most && c.T * parts * 2 <= room && c.Vl / per_vec >= (int64_t)DT * parts * 2) parts *= 2;
+  return parts;
+}
+// CTAs of a launch: one per row and part; as many as fit on the SMs of a budget, which then walk over the rows.
+static unsigned int d_grid(const DistillCall& c, int parts) {
+  const int sms = dh_sm_count();
+  int64_t rows = c.T;
+  if (c.budget > 0 && c.budget < sms) {
+    const int64_t fit = 4 * c.budget / parts;
+    rows = rows < fit ? rows : fit < 1 ? 1 : fit;
+  }
+  const int64_t most = INT32_MAX / parts;
+  return (unsigned int)((rows < most ? rows : most) * parts);
+}
+
+template <typename T>
+static cudaError_t d_launch_fwd(const DistillCall& c, float* ce, float* kd, float4* saved, float4* stats) {
+  void (*const kernels[4])(const DistillArgs, int, float*, float*, float4*, float4*) = {
+      distill_fwd_kernel<T, D_ONE>, distill_fwd_kernel<T, D_TWO>, distill_fwd_kernel<T, D_SQUARE>, distill_fwd_kernel<T, D_FOURTH>};
+  const int parts = d_parts(c, DVec<T>::N, 8);       // the largest cluster that every GPU runs
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(d_grid(c, parts));
+  cfg.blockDim = dim3(DT);
+  cfg.stream = (cudaStream_t)c.stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = parts > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernels[d_mode(c)], d_args(c), parts, ce, kd, saved, stats);
+}
+template <typename T>
+static void d_launch_bwd(const DistillCall& c, const float4* saved, const float* g_ce, const float* g_kd, void* out, int64_t out_ld) {
+  void (*const kernels[4])(const DistillArgs, int, const float4*, const float*, const float*, void*, int64_t) = {
+      distill_bwd_kernel<T, D_ONE>, distill_bwd_kernel<T, D_TWO>, distill_bwd_kernel<T, D_SQUARE>, distill_bwd_kernel<T, D_FOURTH>};
+  const int parts = d_parts(c, DVec<T>::N, 64);
+  kernels[d_mode(c)]<<<d_grid(c, parts), DT, 0, (cudaStream_t)c.stream>>>(d_args(c), parts, saved, g_ce, g_kd, out, out_ld);
 }
 
 }  // namespace dh
@@ -256,32 +573,27 @@ using namespace dh;
 
 extern "C" {
 
-// stats [T, 8] and teacher_lse [T], fp32; logits bf16 or fp32 (f32).
-int dh_distill_stats(const void* z, int64_t ld, int f32, const void* labels, const void* ids, int64_t id_stride, int id64, const void* t,
-                     int64_t t_stride, int t_type, int T, int Vl, int K, int v0, int V, float tau, void* stats, void* teacher_lse, int sm_budget,
-                     cudaStream_t s) {
-  if (int rc = d_refuse("dh_distill_stats", T, Vl, K, v0, V, 1.f / tau)) return rc;
-  if (T == 0) return 0;
-  const DistillArgs a{z, ld, (const int*)labels, ids, id_stride, t, t_stride, id64, t_type, T, Vl, K, v0, V, 1.f / tau};
-  if (f32) distill_stats_kernel<float><<<d_grid(T, sm_budget), DT, 0, s>>>(a, (float*)stats, (float*)teacher_lse);
-  else distill_stats_kernel<__nv_bfloat16><<<d_grid(T, sm_budget), DT, 0, s>>>(a, (float*)stats, (float*)teacher_lse);
-  return d_rc("dh_distill_stats");
+// ce [T] (null without labels), kd [T], saved [T, 4] fp32; or, for a shard of a divided vocabulary, stats [T, 8] alone.
+int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stats) {
+  const DistillCall& c = *(const DistillCall*)call;
+  if (int rc = d_refuse("dh_distill_fwd", c)) return rc;
+  if (c.T == 0) return 0;
+  const cudaError_t e = c.f32 ? d_launch_fwd<float>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats)
+                              : d_launch_fwd<__nv_bfloat16>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats);
+  return d_rc("dh_distill_fwd", e);
 }
-int dh_distill_combine(const void* stats, const void* teacher_lse, int R, int T, float tau, void* ce, void* kd, void* saved, cudaStream_t s) {
+int dh_distill_combine(const void* stats, int R, int T, float tau, void* ce, void* kd, void* saved, cudaStream_t s) {
   if (R <= 0 || T <= 0) return 0;
-  distill_combine_kernel<<<(T + DT - 1) / DT, DT, 0, s>>>((const float4*)stats, (const float*)teacher_lse, R, T, tau, (float*)ce, (float*)kd,
-                                                          (float4*)saved);
-  return d_rc("dh_distill_combine");
+  distill_combine_kernel<<<(T + DT - 1) / DT, DT, 0, s>>>((const float4*)stats, R, T, tau, (float*)ce, (float*)kd, (float4*)saved);
+  return d_rc("dh_distill_combine", cudaSuccess);
 }
-int dh_distill_grad(const void* z, int64_t ld, int f32, const void* labels, const void* ids, int64_t id_stride, int id64, const void* t,
-                    int64_t t_stride, int t_type, int T, int Vl, int K, int v0, int V, float tau, const void* saved, const void* g_ce,
-                    const void* g_kd, void* out, int64_t out_ld, int sm_budget, cudaStream_t s) {
-  if (int rc = d_refuse("dh_distill_grad", T, Vl, K, v0, V, 1.f / tau)) return rc;
-  if (T == 0) return 0;
-  const DistillArgs a{z, ld, (const int*)labels, ids, id_stride, t, t_stride, id64, t_type, T, Vl, K, v0, V, 1.f / tau};
-  if (f32) distill_grad_kernel<float><<<d_grid(T, sm_budget), DT, 0, s>>>(a, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, tau, out, out_ld);
-  else distill_grad_kernel<__nv_bfloat16><<<d_grid(T, sm_budget), DT, 0, s>>>(a, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, tau, out, out_ld);
-  return d_rc("dh_distill_grad");
+int dh_distill_bwd(const void* call, const void* saved, const void* g_ce, const void* g_kd, void* out, int64_t out_ld) {
+  const DistillCall& c = *(const DistillCall*)call;
+  if (int rc = d_refuse("dh_distill_bwd", c)) return rc;
+  if (c.T == 0) return 0;
+  if (c.f32) d_launch_bwd<float>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);
+  else d_launch_bwd<__nv_bfloat16>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);
+  return d_rc("dh_distill_bwd", cudaSuccess);
 }
 
 }  // extern "C"

@@ -16,6 +16,7 @@ depend on the tensor-parallel size.
 """
 from __future__ import annotations
 
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 
 import torch
@@ -143,15 +144,16 @@ def _distill_native(what, logits, labels, top_ids, top_logits, *others):
             top_logits if top_logits.stride(1) == 1 else top_logits.contiguous())
 
 
-_DISTILL_OPERANDS = [c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_int, c_int,
-                     c_float]
+# The operands of both kernels as one block of 8-byte fields (DistillCall in csrc/distill.cu): ctypes converts argument by argument,
+# which takes 2 us where a small call has 12 in all.
+_DISTILL_CALL = struct.Struct("=17qd")
 
 
-def _distill_arguments(logits, labels, ids, top, vocab_start, vocab, temperature):
+def _distill_call(logits, labels, ids, top, vocab_start, vocab, temperature, sm_budget):
     T, Vl = logits.shape
-    return (logits.data_ptr(), logits.stride(0), int(logits.dtype == torch.float32), K.ptr(labels), ids.data_ptr(), ids.stride(0),
-            int(ids.dtype == torch.int64), top.data_ptr(), top.stride(0), _TEACHER_TYPES[top.dtype], T, Vl, ids.shape[1], vocab_start, vocab,
-            temperature)
+    return _DISTILL_CALL.pack(logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32, K.ptr(labels), ids.data_ptr(), ids.stride(0),
+                              ids.dtype == torch.int64, top.data_ptr(), top.stride(0), _TEACHER_TYPES[top.dtype], T, Vl, ids.shape[1],
+                              vocab_start, vocab, sm_budget, K.current_raw_stream(), temperature)
 
 
 def _teacher_ref(top_ids, top_logits, vocab, temperature):
@@ -166,6 +168,8 @@ def _teacher_ref(top_ids, top_logits, vocab, temperature):
 
 
 def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature):
+    """``[T, 8]``: maximum m, sums of exp(z - m) and exp((z - m) / tau), z_label - m (+inf: the label is not here), sums of q (z_id - m) / tau
+    and q over the entries here, sum of q log q (+inf: the row has no entries), the teacher's log-sum-exp."""
     Vl = logits.shape[1]
     lf = logits.float()
     m = lf.max(dim=-1).values.clamp_min(torch.finfo(torch.float32).min)
@@ -173,36 +177,32 @@ def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, 
     q, t_lse = _teacher_ref(top_ids, top_logits, vocab, temperature)
     loc = top_ids.long() - vocab_start
     own = (loc >= 0) & (loc < Vl) & (q != 0)
-    zero = torch.zeros_like(q)
-    dot = torch.where(own, q * rel.gather(1, loc.clamp(0, Vl - 1)), zero).sum(1)
+    zero, inf = torch.zeros_like(q), torch.full_like(m, float("inf"))
+    dot = torch.where(own, q * rel.gather(1, loc.clamp(0, Vl - 1)), zero).sum(1) / temperature
     ent = torch.where(q != 0, q * torch.log(torch.where(q != 0, q, 1.0)), zero).sum(1)
-    has = torch.zeros_like(m)
-    target = torch.zeros_like(m)
+    target = inf
     if labels is not None:
         loc = labels.long() - vocab_start
         inside = (labels >= 0) & (labels < vocab) & (loc >= 0) & (loc < Vl)
-        has = inside.float()
-        target = torch.where(inside, rel.gather(1, loc.clamp(0, Vl - 1)[:, None]).squeeze(1), target)
-    stats = torch.stack([m, torch.exp(rel).sum(1), torch.exp(rel / temperature).sum(1), target, dot, torch.where(own, q, zero).sum(1),
-                         torch.where(torch.isinf(t_lse) & (t_lse > 0), t_lse, ent), has], dim=1)
-    return stats, t_lse
+        target = torch.where(inside, rel.gather(1, loc.clamp(0, Vl - 1)[:, None]).squeeze(1), inf)
+    return torch.stack([m, torch.exp(rel).sum(1), torch.exp(rel / temperature).sum(1), target, dot, torch.where(own, q, zero).sum(1),
+                        torch.where(t_lse == inf, inf, ent), t_lse], dim=1)
 
 
-def _distill_combine_ref(all_stats, t_lse, temperature, hard):
+def _distill_combine_ref(all_stats, temperature, hard):
     m = all_stats[..., 0].max(dim=0).values
-    d = all_stats[..., 0] - m
-    lse = torch.log((all_stats[..., 1] * torch.exp(d)).sum(0))
-    lse_t = torch.log((all_stats[..., 2] * torch.exp(d / temperature)).sum(0))
-    seen = (all_stats[..., 1] != 0).any(0)                   # some logit of the row is not -inf
-    has, own = all_stats[..., 7] != 0, all_stats[..., 5]
-    target = torch.where(has, all_stats[..., 3] + d, 0.0).sum(0)
-    dot = torch.where(own != 0, all_stats[..., 4] + own * d, 0.0).sum(0)
-    ent = all_stats[0, :, 6]
-    is_hard, is_soft = has.any(0) & seen, (ent != float("inf")) & seen
-    ce = torch.where(is_hard, lse - target, 0.0) if hard else None
-    kd = torch.where(is_soft, temperature ** 2 * (ent - dot / temperature + lse_t), 0.0)
     inf = torch.full_like(m, float("inf"))
-    return ce, kd, torch.stack([m, torch.where(is_hard, lse + m, inf), lse_t + m / temperature, torch.where(is_soft, t_lse, inf)], dim=1)
+    d = all_stats[..., 0] - m
+    s1 = (all_stats[..., 1] * torch.exp(d)).sum(0)
+    st = (all_stats[..., 2] * torch.exp(d / temperature)).sum(0)
+    has, own, ent = all_stats[..., 3] != inf, all_stats[..., 5], all_stats[0, :, 6]
+    target = torch.where(has, all_stats[..., 3] + d, 0.0).sum(0)
+    dot = torch.where(own != 0, all_stats[..., 4] + own * (d / temperature), 0.0).sum(0)
+    is_hard, is_soft = has.any(0) & (s1 != 0), (ent != inf) & (st != 0)       # a sum of 0: all logits of the row are -inf
+    ce = torch.where(is_hard, torch.log(s1) - target, 0.0) if hard else None
+    kd = torch.where(is_soft, temperature ** 2 * (ent - dot + torch.log(st)), 0.0)
+    return ce, kd, torch.stack([m, torch.where(is_hard, 1.0 / s1, 0.0), torch.where(is_soft, 1.0 / st, 0.0),
+                                torch.where(is_soft, all_stats[0, :, 7], inf)], dim=1)
 
 
 def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature: float = 1.0, vocab_start: int = 0, group=None,
@@ -229,26 +229,26 @@ def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature:
     native = K.use_native(logits)
     if native:
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits)
-        stats = torch.empty((T, 8), dtype=torch.float32, device=logits.device)
-        t_lse = torch.empty(T, dtype=torch.float32, device=logits.device)
-        fn = K.proto("dh_distill_stats", _DISTILL_OPERANDS + [c_void_p, c_void_p, c_int, c_void_p])
-        K.check(fn(*_distill_arguments(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature), stats.data_ptr(),
-                   t_lse.data_ptr(), sm_budget, K.stream_ptr()), "dh_distill_stats")
+        call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature, sm_budget)
+        fn = K.proto("dh_distill_fwd", [c_void_p] * 5)
+        kd = logits.new_empty(T, dtype=torch.float32)
+        ce = torch.empty_like(kd) if labels is not None else None
+        saved = logits.new_empty((T, 4), dtype=torch.float32)
+        if ws == 1:
+            K.check(fn(call, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), 0), what)
+            return ce, kd, saved
+        stats = logits.new_empty((T, 8), dtype=torch.float32)
+        K.check(fn(call, 0, 0, 0, stats.data_ptr()), what)
     else:
-        stats, t_lse = _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature)
+        stats = _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature)
+    every = stats
     if ws > 1:
         every = torch.empty((ws * T, 8), dtype=stats.dtype, device=stats.device)
         dist.all_gather_into_tensor(every, stats, group=group)
-    else:
-        every = stats
     if not native:
-        return _distill_combine_ref(every.view(ws, T, 8), t_lse, temperature, labels is not None)
-    ce = torch.empty(T, dtype=torch.float32, device=logits.device) if labels is not None else None
-    kd = torch.empty(T, dtype=torch.float32, device=logits.device)
-    saved = torch.empty((T, 4), dtype=torch.float32, device=logits.device)
-    fn = K.proto("dh_distill_combine", [c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
-    K.check(fn(every.data_ptr(), t_lse.data_ptr(), ws, T, temperature, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), K.stream_ptr()),
-            "dh_distill_combine")
+        return _distill_combine_ref(every.view(ws, T, 8), temperature, labels is not None)
+    fn = K.proto("dh_distill_combine", [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
+    K.check(fn(every.data_ptr(), ws, T, temperature, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), K.stream_ptr()), what)
     return ce, kd, saved
 
 
@@ -276,23 +276,22 @@ def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce
             raise ValueError(f"{what}: contiguous fp32 gradients [T] and saved statistics [T, 4], got {t.dtype} {tuple(t.shape)}")
     if K.use_native(logits):
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out)
-        fn = K.proto("dh_distill_grad", _DISTILL_OPERANDS + [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int, c_void_p])
-        K.check(fn(*_distill_arguments(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature), saved.data_ptr(),
-                   K.ptr(g_ce), g_kd.data_ptr(), out.data_ptr(), out.stride(0), sm_budget, K.stream_ptr()), "dh_distill_grad")
+        call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature, sm_budget)
+        fn = K.proto("dh_distill_bwd", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64])
+        K.check(fn(call, saved.data_ptr(), K.ptr(g_ce), g_kd.data_ptr(), out.data_ptr(), out.stride(0)), what)
         return out
-    lf = logits.float()
-    lse, lse_t, t_lse = saved[:, 1:2], saved[:, 2:3], saved[:, 3:4]
-    some = t_lse.squeeze(1) != float("inf")
-    gk = torch.where(some, g_kd, 0.0) * temperature
-    d = torch.where(gk[:, None] != 0, torch.exp(lf / temperature - lse_t) * gk[:, None], 0.0)
+    rel = logits.float() - saved[:, :1]
+    inv, inv_t, t_lse = saved[:, 1], saved[:, 2], saved[:, 3]
+    gk = torch.where(t_lse != float("inf"), g_kd, 0.0) * temperature
+    d = torch.where(gk[:, None] != 0, torch.exp(rel / temperature) * (gk * inv_t)[:, None], 0.0)
     loc = top_ids.long() - vocab_start
     own = (loc >= 0) & (loc < Vl) & (gk[:, None] != 0)
-    w = torch.where(own, torch.exp(top_logits.float() / temperature - t_lse) * gk[:, None], 0.0)
+    w = torch.where(own, torch.exp(top_logits.float() / temperature - t_lse[:, None]) * gk[:, None], 0.0)
     d.scatter_add_(1, loc.clamp(0, Vl - 1), -w)
     if labels is not None:
         loc = labels.long() - vocab_start
-        gc = torch.where(lse.squeeze(1) != float("inf"), g_ce, 0.0)
-        d = d + torch.where(gc[:, None] != 0, torch.exp(lf - lse) * gc[:, None], 0.0)
+        gc = torch.where(inv != 0, g_ce, 0.0)
+        d = d + torch.where(gc[:, None] != 0, torch.exp(rel) * (gc * inv)[:, None], 0.0)
         own = (loc >= 0) & (loc < Vl)
         d.scatter_add_(1, loc.clamp(0, Vl - 1)[:, None], torch.where(own, -gc, 0.0)[:, None])
     return out.copy_(d.to(out.dtype))

@@ -333,26 +333,22 @@ def test_distill_infinities_and_nan():
     assert float(run_distill(case, 2.0)[2][1].abs().max()) == 0.0
 
 
-def test_distill_rows_of_a_shard_and_their_combination():
-    """The statistics of two shards, as two ranks would exchange them, give what the whole row gives."""
-    from dhellam_b200 import kernels as K
+@pytest.mark.parametrize("tau", [1.0, 1.4, 2.0])
+def test_distill_rows_of_shards_and_their_combination(tau, monkeypatch):
+    """Two ranks' calls one after the other, with the exchange between them replaced by what the two calls send."""
     case = distill_case(17, 4010, 12, seed=4, dtype=BF)
     z, labels, ids, top, g_ce, g_kd = on_gpu(case)
-    tau, v1 = 1.4, 2005
-    halves, lse = [], None
-    for v0 in (0, v1):
-        part = z[:, v0:v0 + v1]
-        st, lse = torch.empty(17, 8, device=DEV), torch.empty(17, device=DEV)
-        fn = K.proto("dh_distill_stats", L._DISTILL_OPERANDS + [L.c_void_p, L.c_void_p, L.c_int, L.c_void_p])
-        K.check(fn(*L._distill_arguments(part, labels, ids, top, v0, 4010, tau), st.data_ptr(), lse.data_ptr(), 0, K.stream_ptr()))
-        halves.append(st)
-    ce, kd, saved = torch.empty(17, device=DEV), torch.empty(17, device=DEV), torch.empty(17, 4, device=DEV)
-    every = torch.stack(halves)
-    fn = K.proto("dh_distill_combine", [L.c_void_p, L.c_void_p, L.c_int, L.c_int, L.c_float, L.c_void_p, L.c_void_p, L.c_void_p, L.c_void_p])
-    K.check(fn(every.data_ptr(), lse.data_ptr(), 2, 17, tau, ce.data_ptr(), kd.data_ptr(), saved.data_ptr(), K.stream_ptr()))
+    sent = []
+    monkeypatch.setattr(L, "group_size", lambda group: 2)
+    monkeypatch.setattr(L.dist, "all_gather_into_tensor", lambda every, stats, group=None: sent.append(stats.clone()))
+    for v0 in (0, 2005):
+        L.vocab_parallel_distill_fwd(z[:, v0:v0 + 2005], labels, ids, top, tau, vocab_start=v0)
+    monkeypatch.setattr(L.dist, "all_gather_into_tensor", lambda every, stats, group=None: every.copy_(torch.cat(sent)))
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z[:, :2005], labels, ids, top, tau)
     grad = torch.empty_like(z)
-    for v0 in (0, v1):
-        L.vocab_parallel_distill_bwd_(z[:, v0:v0 + v1], labels, ids, top, saved, g_ce, g_kd, tau, vocab_start=v0, out=grad[:, v0:v0 + v1])
+    for v0 in (0, 2005):
+        part = slice(v0, v0 + 2005)
+        L.vocab_parallel_distill_bwd_(z[:, part], labels, ids, top, saved, g_ce, g_kd, tau, vocab_start=v0, out=grad[:, part])
     check_distill(case, tau, ce, kd, grad, BF)
 
 
