@@ -22,6 +22,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <float.h>
+#include <limits.h>
 #include <math.h>
 #include <stdint.h>
 
@@ -31,9 +32,8 @@
 
 namespace dh {
 
-constexpr int DT = 256;                  // threads of a CTA
-constexpr int DW = DT / 32;
 constexpr int D_MAX_K = 1024;
+constexpr int D_TABLE = 4096;            // slots for the entries of a row in the backward
 constexpr int D_BATCH = 4;               // 16-byte loads of a thread in flight
 constexpr float D_LOG2E = 1.4426950408889634f;
 constexpr float D_LN2 = 0.6931471805599453f;
@@ -102,6 +102,23 @@ __device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
 __device__ __forceinline__ F2 f2_ex2(F2 a) {
   const float2 x = f2_get(a);
   return f2(d_ex2(x.x), d_ex2(x.y));
+}
+
+// 2^x on the FMA pipe, for x up to 126 and (as 2^-126) below -126: x = n + f with |f| <= 1/2 by adding 1.5 x 2^23, a polynomial of degree 5
+// for 2^f (own minimax fit by Remez' exchange, relative error 2.1e-7 in fp32, the special function's bound is 2.4e-7), n added to the
+// exponent.  NaN is lost.
+__device__ __forceinline__ F2 f2_ex2_fma(F2 a) {
+  const float2 x = f2_get(a);
+  const F2 c = f2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const F2 t = c + f2(12582912.f, 12582912.f);
+  const F2 f = f2_fma(t + f2(-12582912.f, -12582912.f), f2(-1.f, -1.f), c);
+  F2 p = f2_fma(f, f2(0.0013277939287945628f, 0.0013277939287945628f), f2(0.009675757959485054f, 0.009675757959485054f));
+  p = f2_fma(p, f, f2(0.05550709739327431f, 0.05550709739327431f));
+  p = f2_fma(p, f, f2(0.24022114276885986f, 0.24022114276885986f));
+  p = f2_fma(p, f, f2(0.6931469440460205f, 0.6931469440460205f));
+  p = f2_fma(p, f, f2(1.0000001192092896f, 1.0000001192092896f));
+  const float2 n = f2_get(t), q = f2_get(p);
+  return f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
 }
 
 // 16 bytes of logits as pairs of fp32, and their largest.
@@ -200,11 +217,13 @@ struct DSums {
     }
     m = to;
   }
+  // FMA: the second of two exponentials on the FMA pipe (whoever asks for it puts NaN back from the first)
+  template <bool FMA>
   __device__ __forceinline__ void add(F2 z, F2 nm, F2 c1, F2 ct) {
     const F2 x = z + nm;
     const F2 e = f2_ex2(x * ct);
     st = st + e;
-    if (MODE == D_TWO) s1 = s1 + f2_ex2(x * c1);
+    if (MODE == D_TWO) s1 = s1 + (FMA ? f2_ex2_fma(x * c1) : f2_ex2(x * c1));
     if (MODE == D_SQUARE) s1 = f2_fma(e, e, s1);
     if (MODE == D_FOURTH) { const F2 q = e * e; s1 = f2_fma(q, q, s1); }
   }
@@ -222,10 +241,10 @@ __device__ __forceinline__ void d_finish(float m, float s1, float st, float targ
 
 // One cluster of CTAs per row (one CTA where there are rows enough); they share its vectors and the first one joins their sums.
 // Where `stats` is given (the vocabulary is divided among ranks) a row's eight numbers go there: m, s1, st, target, dot, own, ent, tl.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a, int parts, float* __restrict__ ce, float* __restrict__ kd,
+template <typename T, int MODE, int DT>
+__global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const DistillArgs a, int parts, float* __restrict__ ce, float* __restrict__ kd,
                                                             float4* __restrict__ saved, float4* __restrict__ stats) {
-  constexpr int N = DVec<T>::N;
+  constexpr int N = DVec<T>::N, DW = DT / 32;
   __shared__ float red[2][DW];
   __shared__ float sums[DW][6];
   __shared__ float join[4];                          // this CTA's m, s1, st for the first one of its cluster
@@ -238,8 +257,23 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
     const DSpan sp = d_span(z, a.Vl, part, parts);
     const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
+    // what a row's end needs is on its way before its logits are
+    int id0 = -1, lab = -1;
+    float t0 = 0.f;
+    if (part == 0) {
+      if ((int)threadIdx.x < a.K) { id0 = d_id(a, row, threadIdx.x); t0 = d_teacher(a, row, threadIdx.x); }
+      if (threadIdx.x == 0 && a.labels != nullptr) lab = a.labels[row];
+    }
     DSums<MODE> acc;
     F2 x[N / 2];
+    auto take = [&](const uint4& u, F2 nm) {
+      DVec<T>::unpack(u, x);
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        if (j % 2 == 1 && N == 8) acc.template add<true>(x[j], nm, c1p, ctp);
+        else acc.template add<false>(x[j], nm, c1p, ctp);
+      }
+    };
     int i = sp.v0 + threadIdx.x;
     for (; i + (D_BATCH - 1) * DT < sp.v1; i += D_BATCH * DT) {
       uint4 u[D_BATCH];
@@ -249,11 +283,7 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
       if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
       const F2 nm = f2(-acc.m, -acc.m);
 #pragma unroll
-      for (int b = 0; b < D_BATCH; ++b) {
-        DVec<T>::unpack(u[b], x);
-#pragma unroll
-        for (int j = 0; j < N / 2; ++j) acc.add(x[j], nm, c1p, ctp);
-      }
+      for (int b = 0; b < D_BATCH; ++b) take(u[b], nm);
     }
     for (; i < sp.v1; i += DT) {
       uint4 u[D_BATCH];
@@ -262,16 +292,17 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
       for (int b = 1; b < D_BATCH; ++b) u[b] = u[0];
       const float lm = DVec<T>::largest(u);
       if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
-      const F2 nm = f2(-acc.m, -acc.m);
-      DVec<T>::unpack(u[0], x);
-#pragma unroll
-      for (int j = 0; j < N / 2; ++j) acc.add(x[j], nm, c1p, ctp);
+      take(u[0], f2(-acc.m, -acc.m));
     }
+    const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
+    const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
+    const bool lin = lloc >= 0 && lloc < a.Vl;
+    const float zl = lin ? d_load(z + lloc) : 0.f;
     float s1, st;
     {
       const float2 p = f2_get(acc.s1), q = f2_get(acc.st);
-      s1 = p.x + p.y;
       st = q.x + q.y;
+      s1 = MODE == D_TWO ? fmaf(0.f, st, p.x + p.y) : p.x + p.y;      // a NaN that the FMA pipe's exponentials lost is in the other sum
     }
     // elements before the first and behind the last vector
     auto single = [&](int c) {
@@ -288,8 +319,9 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
     if (part == parts - 1 && sp.lead + sp.vecs * N + (int)threadIdx.x < a.Vl) single(sp.lead + sp.vecs * N + threadIdx.x);
     // first round: the CTA's reference and the teacher's largest logit
     float tm = -INFINITY;
+    if (id0 >= 0) tm = t0;
     if (part == 0)
-      for (int j = threadIdx.x; j < a.K; j += DT)
+      for (int j = threadIdx.x + DT; j < a.K; j += DT)
         if (d_id(a, row, j) >= 0) tm = d_max(tm, d_teacher(a, row, j));
     const float wm = d_warp_max(acc.m);
     tm = d_warp_max(tm);
@@ -303,16 +335,17 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
     float v[6] = {s1 * d_ex2((acc.m - m) * c1), st * d_ex2((acc.m - m) * ct), 0.f, 0.f, 0.f, 0.f};
     if (part == 0 && tm != -INFINITY)
       for (int j = threadIdx.x; j < a.K; j += DT) {
-        const int id = d_id(a, row, j);
+        const bool early = j == (int)threadIdx.x;
+        const int id = early ? id0 : d_id(a, row, j);
         if (id < 0) continue;
-        const float lt = (d_teacher(a, row, j) - tm) * a.inv_tau;
+        const float lt = ((early ? t0 : d_teacher(a, row, j)) - tm) * a.inv_tau;
         const float q = expf(lt);
         if (q == 0.f) continue;                          // no weight: its logit may be infinite
         v[2] += q;
         v[3] += q * lt;
         const int loc = id - a.v0;
         if (loc >= 0 && loc < a.Vl) {
-          v[4] += q * ((d_load(z + loc) - m) * ct);
+          v[4] += q * (((early ? z0 : d_load(z + loc)) - m) * ct);
           v[5] += q;
         }
       }
@@ -337,9 +370,7 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
     if (parts > 1) cluster_sync_all();
     if (part == 0 && threadIdx.x == 0) {
       float dot = v[4], own = v[5];
-      const int lab = a.labels != nullptr ? a.labels[row] : -1;
-      const int loc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
-      float target = loc >= 0 && loc < a.Vl ? (d_load(z + loc) - m) * c1 : INFINITY;
+      float target = lin ? (zl - m) * c1 : INFINITY;
       for (int r = 1; r < parts; ++r) {
         const uint32_t at = mapa_u32(smem_u32(join), r);
         const float om = __uint_as_float(ld_cluster_u32(at)), o1 = __uint_as_float(ld_cluster_u32(at + 4)),
@@ -369,9 +400,9 @@ __global__ void __launch_bounds__(DT, 4) distill_fwd_kernel(const DistillArgs a,
 
 // stats [R, T, 8] of the ranks -> ce [T] (nullable), kd [T], saved [T, 4] = (m, 1 / sum or 0 where ce has no gradient, 1 / sum at tau,
 // the teacher's lse at tau or +inf where kd has no gradient).
-__global__ void __launch_bounds__(DT) distill_combine_kernel(const float4* __restrict__ stats, int R, int T, float tau, float* __restrict__ ce,
+__global__ void __launch_bounds__(256) distill_combine_kernel(const float4* __restrict__ stats, int R, int T, float tau, float* __restrict__ ce,
                                                              float* __restrict__ kd, float4* __restrict__ saved) {
-  const int t = blockIdx.x * DT + threadIdx.x;
+  const int t = blockIdx.x * 256 + threadIdx.x;
   if (t >= T) return;
   const float ct = D_LOG2E / tau;
   float m = stats[(size_t)t * 2].x;
@@ -390,23 +421,49 @@ __global__ void __launch_bounds__(DT) distill_combine_kernel(const float4* __res
   d_finish(m, s1, st, target, dot, ent, tl, tau, ce != nullptr ? ce + t : nullptr, kd + t, saved + t);
 }
 
-// out = d loss / d z; out may be z.  One CTA per part of a row.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(DT, 4) distill_bwd_kernel(const DistillArgs a, int parts, const float4* __restrict__ saved,
+__device__ __forceinline__ int d_slot(int id, int slots) { return (int)(((unsigned int)id * 2654435761u) >> 16) & (slots - 1); }
+
+// out = d loss / d z; out may be z.  One CTA per part of a row, last rows first: where the backward follows the forward, the L2 still
+// holds the rows that it read last (and the stores ask not to be kept there).
+template <typename T, int MODE, int DT>
+__global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const DistillArgs a, int parts, const float4* __restrict__ saved,
                                                             const float* __restrict__ g_ce, const float* __restrict__ g_kd, void* out,
-                                                            int64_t out_ld) {
+                                                            int64_t out_ld, int slots) {
   constexpr int N = DVec<T>::N;
-  __shared__ int ids[D_MAX_K + 1];          // entries of this part that get more than the softmax: the teacher's, then the label
-  __shared__ float add[D_MAX_K + 1], at[D_MAX_K + 1];
+  // Entries of this part that get more than the softmax: the teacher's, then the label.  An id may stand twice (often the label among the
+  // teacher's), so the first entry of an id writes for all: `first` has the lowest entry of each hash slot, which settles nearly all
+  // of them; only entries that met another id there, and first entries with twins, look through the list (K^2 steps without it:
+  // 256 entries took 113 of 457 us at 4096 x 128256).
+  extern __shared__ __align__(16) int d_shared[];
+  int* first = d_shared;                    // [slots]
+  int* ids = first + slots;                 // [K + 1], -1: not in this part
+  float* add = reinterpret_cast<float*>(ids + a.K + 1);
+  float* at = add + a.K + 1;
+  int* twins = reinterpret_cast<int*>(at + a.K + 1);
   const int part = blockIdx.x % parts;
   const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
-  for (int row = blockIdx.x / parts; row < a.T; row += gridDim.x / parts) {
+  for (int back = blockIdx.x / parts; back < a.T; back += gridDim.x / parts) {
+    const int row = a.T - 1 - back;
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
     T* o = reinterpret_cast<T*>(out) + row * out_ld;
     const DSpan sp = d_span(z, a.Vl, part, parts);
     const float4 sv = saved[row];
     const float gc = a.labels != nullptr && sv.y != 0.f ? g_ce[row] : 0.f, gk = sv.w != INFINITY ? g_kd[row] * a.tau : 0.f;
     const float A = gc != 0.f ? gc * sv.y : 0.f, B = gk != 0.f ? gk * sv.z : 0.f;
+    const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
+    const bool zero = gc == 0.f && gk == 0.f;        // a token without loss: zeros, whatever its logits
+    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
+    uint4* ov = reinterpret_cast<uint4*>(o + sp.lead);
+    // the first logits are on their way before the entries are
+    int i = sp.v0 + threadIdx.x;
+    uint4 u[D_BATCH];
+    const bool ahead = same && !zero && i + (D_BATCH - 1) * DT < sp.v1;
+    if (ahead) {
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b) u[b] = zv[i + b * DT];
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < slots / 4; j += DT) reinterpret_cast<int4*>(first)[j] = make_int4(INT_MAX, INT_MAX, INT_MAX, INT_MAX);
     __syncthreads();
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       int loc = -1;
@@ -421,9 +478,14 @@ __global__ void __launch_bounds__(DT, 4) distill_bwd_kernel(const DistillArgs a,
       ids[j] = in ? loc : -1;
       add[j] = g;
       at[j] = in ? d_load(z + loc) : 0.f;
+      twins[j] = 0;
+      if (in) atomicMin(first + d_slot(loc, slots), j);
     }
     __syncthreads();
-    const bool zero = gc == 0.f && gk == 0.f;        // a token without loss: zeros, whatever its logits
+    for (int j = threadIdx.x; j <= a.K; j += DT) {
+      const int id = ids[j], f = id >= 0 ? first[d_slot(id, slots)] : j;
+      if (f != j && ids[f] == id) twins[f] = 1;
+    }
     const F2 nm = f2(-sv.x, -sv.x), c1p = f2(c1, c1), ctp = f2(ct, ct), Ap = f2(A, A), Bp = f2(B, B);
     auto soft2 = [&](F2 v) {
       const F2 x = v + nm;
@@ -435,46 +497,51 @@ __global__ void __launch_bounds__(DT, 4) distill_bwd_kernel(const DistillArgs a,
     };
     auto soft = [&](float v) { return f2_get(soft2(f2(v, v))).x; };
     auto single = [&](int c) { d_store(o + c, zero ? 0.f : soft(d_load(z + c))); };
-    if (((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(o)) & 15) != 0) {
+    if (!same) {
       for (int c = sp.c0 + threadIdx.x; c < sp.c1; c += DT) single(c);      // rows that are aligned differently
     } else {
-      const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
-      uint4* ov = reinterpret_cast<uint4*>(o + sp.lead);
       if (part == 0 && (int)threadIdx.x < sp.lead) single(threadIdx.x);
       if (part == parts - 1 && sp.lead + sp.vecs * N + (int)threadIdx.x < a.Vl) single(sp.lead + sp.vecs * N + threadIdx.x);
       if (zero) {
-        for (int i = sp.v0 + threadIdx.x; i < sp.v1; i += DT) ov[i] = make_uint4(0, 0, 0, 0);
+        for (; i < sp.v1; i += DT) __stcs(ov + i, make_uint4(0, 0, 0, 0));
       } else {
-        auto vec = [&](const uint4& u) {
+        auto vec = [&](const uint4& r) {
           F2 x[N / 2];
-          DVec<T>::unpack(u, x);
+          DVec<T>::unpack(r, x);
 #pragma unroll
           for (int j = 0; j < N / 2; ++j) x[j] = soft2(x[j]);
           return DVec<T>::pack(x);
         };
-        int i = sp.v0 + threadIdx.x;
-        for (; i + (D_BATCH - 1) * DT < sp.v1; i += D_BATCH * DT) {
-          uint4 u[D_BATCH];
+        if (ahead) {
+          while (true) {
 #pragma unroll
-          for (int b = 0; b < D_BATCH; ++b) u[b] = zv[i + b * DT];
+            for (int b = 0; b < D_BATCH; ++b) __stcs(ov + i + b * DT, vec(u[b]));
+            i += D_BATCH * DT;
+            if (i + (D_BATCH - 1) * DT >= sp.v1) break;
 #pragma unroll
-          for (int b = 0; b < D_BATCH; ++b) ov[i + b * DT] = vec(u[b]);
+            for (int b = 0; b < D_BATCH; ++b) u[b] = zv[i + b * DT];
+          }
         }
-        for (; i < sp.v1; i += DT) ov[i] = vec(zv[i]);
+        for (; i < sp.v1; i += DT) __stcs(ov + i, vec(zv[i]));
       }
     }
     __syncthreads();
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       const int id = ids[j];
       if (id < 0 || zero) continue;
-      bool first = true;
+      const int f = first[d_slot(id, slots)];
+      if (f != j && ids[f] == id) continue;             // the first of its id writes for it
       float g = add[j];
-      for (int i = 0; i <= a.K; ++i) {
-        if (i == j || ids[i] != id) continue;
-        if (i < j) first = false;
-        else g += add[i];
+      bool mine = true;
+      if (f != j || twins[j]) {
+        g = 0.f;
+        for (int q = 0; q <= a.K; ++q) {
+          if (ids[q] != id) continue;
+          if (q < j) mine = false;
+          g += add[q];
+        }
       }
-      if (first) d_store(o + id, soft(at[j]) - g);
+      if (mine) d_store(o + id, soft(at[j]) - g);
     }
   }
 }
@@ -522,33 +589,39 @@ static int d_mode(const DistillCall& c) {
   if (c.labels == 0 || c.tau == 1.) return D_ONE;
   return c.tau == 2. ? D_SQUARE : c.tau == 4. ? D_FOURTH : D_TWO;
 }
+// Threads of a CTA: two batches of loads each, as far as 64 to 256 threads give that.  A row has some microseconds of its own (the
+// entries, two rounds of reductions), so short rows take small CTAs and the SM holds more of them.
+static int d_threads(const DistillCall& c, int per_vec) {
+  const int64_t vecs = c.Vl / per_vec;
+  return vecs >= 8 * 256 ? 256 : vecs >= 8 * 128 ? 128 : 64;
+}
 // CTAs that share a row: where there are fewer rows than the GPU holds CTAs, as long as each thread still has a vector.
-static int d_parts(const DistillCall& c, int per_vec, int most) {
+static int d_parts(const DistillCall& c, int threads, int per_vec, int most) {
   const int sms = dh_sm_count();
-  const int64_t room = 4ll * ((c.budget <= 0 || c.budget > sms) ? sms : c.budget);
+  const int64_t room = 1024 / threads * ((c.budget <= 0 || c.budget > sms) ? sms : c.budget);
   int parts = 1;
-  while (parts < most && c.T * parts * 2 <= room && c.Vl / per_vec >= (int64_t)DT * parts * 2) parts *= 2;
+  while (parts < most && c.T * parts * 2 <= room && c.Vl / per_vec >= (int64_t)threads * parts * 2) parts *= 2;
   return parts;
 }
 // CTAs of a launch: one per row and part; as many as fit on the SMs of a budget, which then walk over the rows.
-static unsigned int d_grid(const DistillCall& c, int parts) {
+static unsigned int d_grid(const DistillCall& c, int threads, int parts) {
   const int sms = dh_sm_count();
   int64_t rows = c.T;
   if (c.budget > 0 && c.budget < sms) {
-    const int64_t fit = 4 * c.budget / parts;
+    const int64_t fit = 1024 / threads * c.budget / parts;
     rows = rows < fit ? rows : fit < 1 ? 1 : fit;
   }
   const int64_t most = INT32_MAX / parts;
   return (unsigned int)((rows < most ? rows : most) * parts);
 }
 
-template <typename T>
-static cudaError_t d_launch_fwd(const DistillCall& c, float* ce, float* kd, float4* saved, float4* stats) {
+template <typename T, int DT>
+static cudaError_t d_launch_fwd_as(const DistillCall& c, float* ce, float* kd, float4* saved, float4* stats) {
   void (*const kernels[4])(const DistillArgs, int, float*, float*, float4*, float4*) = {
-      distill_fwd_kernel<T, D_ONE>, distill_fwd_kernel<T, D_TWO>, distill_fwd_kernel<T, D_SQUARE>, distill_fwd_kernel<T, D_FOURTH>};
-  const int parts = d_parts(c, DVec<T>::N, 8);       // the largest cluster that every GPU runs
+      distill_fwd_kernel<T, D_ONE, DT>, distill_fwd_kernel<T, D_TWO, DT>, distill_fwd_kernel<T, D_SQUARE, DT>, distill_fwd_kernel<T, D_FOURTH, DT>};
+  const int parts = d_parts(c, DT, DVec<T>::N, 8);       // the largest cluster that every GPU runs
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(d_grid(c, parts));
+  cfg.gridDim = dim3(d_grid(c, DT, parts));
   cfg.blockDim = dim3(DT);
   cfg.stream = (cudaStream_t)c.stream;
   cudaLaunchAttribute attr[1];
@@ -560,11 +633,27 @@ static cudaError_t d_launch_fwd(const DistillCall& c, float* ce, float* kd, floa
   return cudaLaunchKernelEx(&cfg, kernels[d_mode(c)], d_args(c), parts, ce, kd, saved, stats);
 }
 template <typename T>
+static cudaError_t d_launch_fwd(const DistillCall& c, float* ce, float* kd, float4* saved, float4* stats) {
+  const int threads = d_threads(c, DVec<T>::N);
+  if (threads == 256) return d_launch_fwd_as<T, 256>(c, ce, kd, saved, stats);
+  return threads == 128 ? d_launch_fwd_as<T, 128>(c, ce, kd, saved, stats) : d_launch_fwd_as<T, 64>(c, ce, kd, saved, stats);
+}
+template <typename T, int DT>
+static void d_launch_bwd_as(const DistillCall& c, const float4* saved, const float* g_ce, const float* g_kd, void* out, int64_t out_ld) {
+  void (*const kernels[4])(const DistillArgs, int, const float4*, const float*, const float*, void*, int64_t, int) = {
+      distill_bwd_kernel<T, D_ONE, DT>, distill_bwd_kernel<T, D_TWO, DT>, distill_bwd_kernel<T, D_SQUARE, DT>, distill_bwd_kernel<T, D_FOURTH, DT>};
+  const int parts = d_parts(c, DT, DVec<T>::N, 64);
+  int slots = 64;
+  while (slots < 8 * c.K && slots < D_TABLE) slots *= 2;
+  const size_t shared = sizeof(int) * (slots + 4 * (size_t)(c.K + 1));       // at most 32 KB
+  kernels[d_mode(c)]<<<d_grid(c, DT, parts), DT, shared, (cudaStream_t)c.stream>>>(d_args(c), parts, saved, g_ce, g_kd, out, out_ld, slots);
+}
+template <typename T>
 static void d_launch_bwd(const DistillCall& c, const float4* saved, const float* g_ce, const float* g_kd, void* out, int64_t out_ld) {
-  void (*const kernels[4])(const DistillArgs, int, const float4*, const float*, const float*, void*, int64_t) = {
-      distill_bwd_kernel<T, D_ONE>, distill_bwd_kernel<T, D_TWO>, distill_bwd_kernel<T, D_SQUARE>, distill_bwd_kernel<T, D_FOURTH>};
-  const int parts = d_parts(c, DVec<T>::N, 64);
-  kernels[d_mode(c)]<<<d_grid(c, parts), DT, 0, (cudaStream_t)c.stream>>>(d_args(c), parts, saved, g_ce, g_kd, out, out_ld);
+  const int threads = d_threads(c, DVec<T>::N);
+  if (threads == 256) d_launch_bwd_as<T, 256>(c, saved, g_ce, g_kd, out, out_ld);
+  else if (threads == 128) d_launch_bwd_as<T, 128>(c, saved, g_ce, g_kd, out, out_ld);
+  else d_launch_bwd_as<T, 64>(c, saved, g_ce, g_kd, out, out_ld);
 }
 
 }  // namespace dh
@@ -584,7 +673,7 @@ int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stat
 }
 int dh_distill_combine(const void* stats, int R, int T, float tau, void* ce, void* kd, void* saved, cudaStream_t s) {
   if (R <= 0 || T <= 0) return 0;
-  distill_combine_kernel<<<(T + DT - 1) / DT, DT, 0, s>>>((const float4*)stats, R, T, tau, (float*)ce, (float*)kd, (float4*)saved);
+  distill_combine_kernel<<<(T + 255) / 256, 256, 0, s>>>((const float4*)stats, R, T, tau, (float*)ce, (float*)kd, (float4*)saved);
   return d_rc("dh_distill_combine", cudaSuccess);
 }
 int dh_distill_bwd(const void* call, const void* saved, const void* g_ce, const void* g_kd, void* out, int64_t out_ld) {
