@@ -8,11 +8,12 @@
 // A label outside [0, V) gives ce = 0 and no gradient, a row without entries kd = 0 and none, a row whose logits are all -inf neither
 // loss nor gradient.  An id may stand twice; its weights add.
 //
-// Forward: one pass over the shard.  Every sum of exponentials is relative to a reference m that is a row's maximum or up to
-// D_RISE / log2 e below it: a thread takes the maximum of its first batch and moves it only when an element rises further, so the
-// rescaling leaves the loop and no term is below what its own rounding loses.  Exponentials are 2^((z - m) c) with c = log2 e or
-// log2 e / tau; the difference first, because (z - m) c is then right for the largest and the lowest finite logits too.  The teacher's sums
-// are linear in exp(t / tau), so one CTA needs two rounds of reductions in all.  Sums are fp32.
+// Forward: one pass over the shard.  A thread's sums of exponentials are relative to a reference m that is the maximum of what it has
+// seen or up to D_RISE / log2 e below it: it moves only when an element rises further, so the rescaling leaves the loop and no term is
+// below what its own rounding loses.  Exponentials are 2^(z c - R) in one fma, with c = log2 e or log2 e / tau and R = m c rounded; the
+// rounding of R is taken out of the sum when the thread is done.  A row whose maximum is
+// beyond D_FAR powers of two (the type's lowest value everywhere) has a slow form, the difference first.  The teacher's sums are linear in
+// exp(t / tau), so one CTA needs two rounds of reductions in all.  Sums are fp32.
 // Backward: one pass computes every element from (m, 1 / sum, 1 / sum at tau) and the few entries with a label or a teacher's weight are
 // written once more behind it, from logits read before it, so that each element is rounded once.
 //
@@ -34,9 +35,10 @@ namespace dh {
 
 constexpr int D_MAX_K = 1024;
 constexpr int D_TABLE = 4096;            // slots for the entries of a row in the backward
-constexpr int D_BATCH = 4;               // 16-byte loads of a thread in flight
+constexpr int D_BATCH = 4;               // 16-byte loads of a thread at a time
 constexpr float D_LOG2E = 1.4426950408889634f;
 constexpr float D_LN2 = 0.6931471805599453f;
+constexpr float D_FAR = 2097152.f;       // references of the fast form are that far from zero at most, in powers of two: 1/8 is what R is off by
 constexpr float D_RISE = 8.f;            // in powers of two; 2^-24 of it is what an exponent loses at most by a reference that is too low
 
 // Which exponentials an element needs: ONE (a single sum), TWO (both, on their own), SQUARE and FOURTH (tau = 2, 4).
@@ -53,6 +55,9 @@ struct DistillArgs {
   float tau, inv_tau;
 };
 
+__device__ __forceinline__ void d_copy16(void* to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
 __device__ __forceinline__ float d_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -104,21 +109,26 @@ __device__ __forceinline__ F2 f2_ex2(F2 a) {
   return f2(d_ex2(x.x), d_ex2(x.y));
 }
 
-// 2^x on the FMA pipe, for x up to 126 and (as 2^-126) below -126: x = n + f with |f| <= 1/2 by adding 1.5 x 2^23, a polynomial of degree 5
-// for 2^f (own minimax fit by Remez' exchange, relative error 2.1e-7 in fp32, the special function's bound is 2.4e-7), n added to the
-// exponent.  NaN is lost.
+// 2^x on the FMA pipe, for x up to 127 and (as 2^-126) below -126: x = n + f with |f| <= 1/2 by adding 1.5 x 2^23 (+ 127, so that the sum's
+// low bits are the exponent field of 2^n), and a polynomial of degree 5 for 2^f (own minimax fit by Remez' exchange, relative error
+// 2.1e-7 in fp32; the special function's bound is 2.4e-7).  A NaN stays.
+__device__ __forceinline__ float d_max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ F2 f2_ex2_fma(F2 a) {
   const float2 x = f2_get(a);
-  const F2 c = f2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-  const F2 t = c + f2(12582912.f, 12582912.f);
-  const F2 f = f2_fma(t + f2(-12582912.f, -12582912.f), f2(-1.f, -1.f), c);
+  const F2 c = f2(d_max_nan(x.x, -126.f), d_max_nan(x.y, -126.f));
+  const F2 t = c + f2(12583039.f, 12583039.f);
+  const F2 f = f2_fma(t + f2(-12583039.f, -12583039.f), f2(-1.f, -1.f), c);
   F2 p = f2_fma(f, f2(0.0013277939287945628f, 0.0013277939287945628f), f2(0.009675757959485054f, 0.009675757959485054f));
   p = f2_fma(p, f, f2(0.05550709739327431f, 0.05550709739327431f));
   p = f2_fma(p, f, f2(0.24022114276885986f, 0.24022114276885986f));
   p = f2_fma(p, f, f2(0.6931469440460205f, 0.6931469440460205f));
   p = f2_fma(p, f, f2(1.0000001192092896f, 1.0000001192092896f));
-  const float2 n = f2_get(t), q = f2_get(p);
-  return f2(__int_as_float(__float_as_int(q.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(q.y) + (__float_as_int(n.y) << 23)));
+  const float2 n = f2_get(t);
+  return p * f2(__int_as_float(__float_as_int(n.x) << 23), __int_as_float(__float_as_int(n.y) << 23));
 }
 
 // 16 bytes of logits as pairs of fp32, and their largest.
@@ -206,26 +216,40 @@ __device__ __forceinline__ DSpan d_span(const T* row, int n, int part, int parts
 // Sums of one thread relative to its reference.
 template <int MODE>
 struct DSums {
-  float m = -FLT_MAX;
+  float m, r1, rt;                                 // reference, rounded m c1 and m ct
   F2 s1 = f2(0.f, 0.f), st = f2(0.f, 0.f);         // ONE: st alone
+  __device__ __forceinline__ void refer(float to, float c1, float ct) {
+    m = to;
+    rt = to * ct;
+    r1 = MODE == D_SQUARE ? 2.f * rt : MODE == D_FOURTH ? 4.f * rt : to * c1;
+  }
   __device__ __forceinline__ void raise(float to, float c1, float ct) {
-    const float f = d_ex2((m - to) * ct);
+    const float o1 = r1, ot = rt;
+    refer(to, c1, ct);
+    const float f = d_ex2(ot - rt);
     st = st * f2(f, f);
     if (MODE != D_ONE) {
-      const float g = d_ex2((m - to) * c1);
+      const float g = d_ex2(o1 - r1);
       s1 = s1 * f2(g, g);
     }
-    m = to;
   }
-  // FMA: the second of two exponentials on the FMA pipe (whoever asks for it puts NaN back from the first)
-  template <bool FMA>
-  __device__ __forceinline__ void add(F2 z, F2 nm, F2 c1, F2 ct) {
-    const F2 x = z + nm;
-    const F2 e = f2_ex2(x * ct);
+  // F1: a second exponential of its own on the FMA pipe
+  template <bool F1>
+  __device__ __forceinline__ void add(F2 z, F2 n1, F2 nt, F2 c1, F2 ct) {
+    const F2 e = f2_ex2(f2_fma(z, ct, nt));
     st = st + e;
-    if (MODE == D_TWO) s1 = s1 + (FMA ? f2_ex2_fma(x * c1) : f2_ex2(x * c1));
+    if (MODE == D_TWO) {
+      const F2 x = f2_fma(z, c1, n1);
+      s1 = s1 + (F1 ? f2_ex2_fma(x) : f2_ex2(x));
+    }
     if (MODE == D_SQUARE) s1 = f2_fma(e, e, s1);
     if (MODE == D_FOURTH) { const F2 q = e * e; s1 = f2_fma(q, q, s1); }
+  }
+  // The sums relative to m itself.
+  __device__ __forceinline__ void finish(float c1, float ct, float& a1, float& at) const {
+    const float2 p = f2_get(s1), q = f2_get(st);
+    at = (q.x + q.y) * d_ex2(-fmaf(m, ct, -rt));
+    a1 = MODE == D_ONE ? 0.f : (p.x + p.y) * d_ex2(-fmaf(m, c1, -r1));
   }
 };
 
@@ -239,25 +263,48 @@ __device__ __forceinline__ void d_finish(float m, float s1, float st, float targ
   *saved = make_float4(m, hard ? 1.f / s1 : 0.f, soft ? 1.f / st : 0.f, soft ? tl : INFINITY);
 }
 
-// One cluster of CTAs per row (one CTA where there are rows enough); they share its vectors and the first one joins their sums.
+// One cluster of CTAs per row (one CTA where there are rows enough); they share its vectors and the first one joins their sums.  CTAs
+// that stay and ask for the next row's logits while they reduce are slower (4096 x 128256: 182 us, 207 so): SMs are not equally far from
+// the memory, and whoever is done takes the next row.  Bound by memory: 180 us without the exponentials.
 // Where `stats` is given (the vocabulary is divided among ranks) a row's eight numbers go there: m, s1, st, target, dot, own, ent, tl.
 template <typename T, int MODE, int DT>
 __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const DistillArgs a, int parts, float* __restrict__ ce, float* __restrict__ kd,
                                                             float4* __restrict__ saved, float4* __restrict__ stats) {
-  constexpr int N = DVec<T>::N, DW = DT / 32;
+  constexpr int N = DVec<T>::N, DW = DT / 32, STAGE = D_BATCH * DT;
+  extern __shared__ __align__(16) uint4 d_ring[];          // [2][D_BATCH][DT]: a thread's vectors pass through its own slots
   __shared__ float red[2][DW];
   __shared__ float sums[DW][6];
   __shared__ float join[4];                          // this CTA's m, s1, st for the first one of its cluster
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = blockIdx.x % parts;
   const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
-  const float cr = MODE == D_ONE ? ct : fmaxf(c1, ct);
+  const float cr = MODE == D_ONE ? ct : fmaxf(c1, ct), far = D_FAR / cr;
   const F2 c1p = f2(c1, c1), ctp = f2(ct, ct);
+  uint4* const ring = d_ring + threadIdx.x;
+
+  const uint4* src;                                  // this thread's next vector to ask for
+  int full, left;                                    // batches of which every thread has all vectors, this thread's vectors behind them
+  auto fetch = [&](int k, int stage) {
+    if (k < full) {
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b) d_copy16(ring + stage + b * DT, src + b * DT);
+    } else if (k == full) {
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b)
+        if (b < left) d_copy16(ring + stage + b * DT, src + b * DT);
+    }
+    src += STAGE;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   for (int row = blockIdx.x / parts; row < a.T; row += gridDim.x / parts) {
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
     const DSpan sp = d_span(z, a.Vl, part, parts);
-    const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
-    // what a row's end needs is on its way before its logits are
+    full = (sp.v1 - sp.v0) / STAGE;
+    left = (sp.v1 - (sp.v0 + full * STAGE + (int)threadIdx.x) + DT - 1) / DT;
+    src = reinterpret_cast<const uint4*>(z + sp.lead) + sp.v0 + threadIdx.x;
+    fetch(0, 0);
+    fetch(1, STAGE);
+    // what a row's end needs is on its way before its logits are added up
     int id0 = -1, lab = -1;
     float t0 = 0.f;
     if (part == 0) {
@@ -265,46 +312,43 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
       if (threadIdx.x == 0 && a.labels != nullptr) lab = a.labels[row];
     }
     DSums<MODE> acc;
-    F2 x[N / 2];
-    auto take = [&](const uint4& u, F2 nm) {
-      DVec<T>::unpack(u, x);
+    acc.refer(-far, c1, ct);               // what lies below counts only where nothing lies above: the slow form
+    auto batch = [&](int stage, int count) {
+      uint4 u[D_BATCH];
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) {
-        if (j % 2 == 1 && N == 8) acc.template add<true>(x[j], nm, c1p, ctp);
-        else acc.template add<false>(x[j], nm, c1p, ctp);
+      for (int b = 0; b < D_BATCH; ++b) u[b] = ring[stage + (b < count ? b : 0) * DT];
+      const float lm = DVec<T>::largest(u);
+      if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
+      const F2 n1 = f2(-acc.r1, -acc.r1), nt = f2(-acc.rt, -acc.rt);
+#pragma unroll
+      for (int b = 0; b < D_BATCH; ++b) {
+        if (b >= count) continue;
+        F2 x[N / 2];
+        DVec<T>::unpack(u[b], x);
+#pragma unroll
+        for (int j = 0; j < N / 2; ++j) {
+          // of two exponentials of their own a quarter goes to the FMA pipe: none, 1/8, 1/4, 3/8 of them 264, 246, 238, 256 us
+          // (4096 x 128256, tau 1.5); of a single one none (a quarter: 182 -> 195 us)
+          if (N == 8 && j < 2) acc.template add<true>(x[j], n1, nt, c1p, ctp);
+          else acc.template add<false>(x[j], n1, nt, c1p, ctp);
+        }
       }
     };
-    int i = sp.v0 + threadIdx.x;
-    for (; i + (D_BATCH - 1) * DT < sp.v1; i += D_BATCH * DT) {
-      uint4 u[D_BATCH];
-#pragma unroll
-      for (int b = 0; b < D_BATCH; ++b) u[b] = ld_nc_v4(zv + i + b * DT);
-      const float lm = DVec<T>::largest(u);
-      if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
-      const F2 nm = f2(-acc.m, -acc.m);
-#pragma unroll
-      for (int b = 0; b < D_BATCH; ++b) take(u[b], nm);
+    int stage = 0;
+    for (int k = 0; k < full; ++k, stage = STAGE - stage) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      batch(stage, D_BATCH);
+      fetch(k + 2, stage);
     }
-    for (; i < sp.v1; i += DT) {
-      uint4 u[D_BATCH];
-      u[0] = ld_nc_v4(zv + i);
-#pragma unroll
-      for (int b = 1; b < D_BATCH; ++b) u[b] = u[0];
-      const float lm = DVec<T>::largest(u);
-      if ((lm - acc.m) * cr > D_RISE) acc.raise(lm, c1, ct);
-      take(u[0], f2(-acc.m, -acc.m));
-    }
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (left > 0) batch(stage, left);
     const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
     const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
     const bool lin = lloc >= 0 && lloc < a.Vl;
     const float zl = lin ? d_load(z + lloc) : 0.f;
     float s1, st;
-    {
-      const float2 p = f2_get(acc.s1), q = f2_get(acc.st);
-      st = q.x + q.y;
-      s1 = MODE == D_TWO ? fmaf(0.f, st, p.x + p.y) : p.x + p.y;      // a NaN that the FMA pipe's exponentials lost is in the other sum
-    }
-    // elements before the first and behind the last vector
+    acc.finish(c1, ct, s1, st);
+    // elements one by one: before the first and behind the last vector
     auto single = [&](int c) {
       const float v = d_load(z + c);
       if ((v - acc.m) * cr > D_RISE) {
@@ -315,22 +359,34 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
       st += d_ex2((v - acc.m) * ct);
       if (MODE != D_ONE) s1 += d_ex2((v - acc.m) * c1);
     };
+    const int tail = sp.lead + sp.vecs * N + (int)threadIdx.x;
     if (part == 0 && (int)threadIdx.x < sp.lead) single(threadIdx.x);
-    if (part == parts - 1 && sp.lead + sp.vecs * N + (int)threadIdx.x < a.Vl) single(sp.lead + sp.vecs * N + threadIdx.x);
+    if (part == parts - 1 && tail < a.Vl) single(tail);
     // first round: the CTA's reference and the teacher's largest logit
     float tm = -INFINITY;
     if (id0 >= 0) tm = t0;
     if (part == 0)
       for (int j = threadIdx.x + DT; j < a.K; j += DT)
         if (d_id(a, row, j) >= 0) tm = d_max(tm, d_teacher(a, row, j));
-    const float wm = d_warp_max(acc.m);
-    tm = d_warp_max(tm);
-    if (lane == 0) { red[0][w] = wm; red[1][w] = tm; }
-    __syncthreads();
-    float m = red[0][0];
-    tm = red[1][0];
+    float m, top;
+    auto round = [&]() {
+      const float wm = d_warp_max(acc.m), wt = d_warp_max(tm);
+      if (lane == 0) { red[0][w] = wm; red[1][w] = wt; }
+      __syncthreads();
+      m = red[0][0];
+      top = red[1][0];
 #pragma unroll
-    for (int q = 1; q < DW; ++q) { m = d_max(m, red[0][q]); tm = d_max(tm, red[1][q]); }
+      for (int q = 1; q < DW; ++q) { m = d_max(m, red[0][q]); top = d_max(top, red[1][q]); }
+    };
+    round();
+    if (!(m > -far && m < far)) {
+      acc.m = -FLT_MAX;
+      s1 = st = 0.f;
+      for (int c = sp.c0 + threadIdx.x; c < sp.c1; c += DT) single(c);
+      __syncthreads();
+      round();
+    }
+    tm = top;
     // second round: the sums; the teacher's relative to its largest
     float v[6] = {s1 * d_ex2((acc.m - m) * c1), st * d_ex2((acc.m - m) * ct), 0.f, 0.f, 0.f, 0.f};
     if (part == 0 && tm != -INFINITY)
@@ -606,13 +662,10 @@ static int d_parts(const DistillCall& c, int threads, int per_vec, int most) {
 // CTAs of a launch: one per row and part; as many as fit on the SMs of a budget, which then walk over the rows.
 static unsigned int d_grid(const DistillCall& c, int threads, int parts) {
   const int sms = dh_sm_count();
-  int64_t rows = c.T;
-  if (c.budget > 0 && c.budget < sms) {
-    const int64_t fit = 1024 / threads * c.budget / parts;
-    rows = rows < fit ? rows : fit < 1 ? 1 : fit;
-  }
-  const int64_t most = INT32_MAX / parts;
-  return (unsigned int)((rows < most ? rows : most) * parts);
+  int64_t fit = INT32_MAX / parts;
+  if (c.budget > 0 && c.budget < sms) fit = 1024 / threads * c.budget / parts;
+  if (fit < 1) fit = 1;
+  return (unsigned int)((c.T < fit ? c.T : fit) * parts);
 }
 
 template <typename T, int DT>
@@ -623,6 +676,7 @@ static cudaError_t d_launch_fwd_as(const DistillCall& c, float* ce, float* kd, f
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(d_grid(c, DT, parts));
   cfg.blockDim = dim3(DT);
+  cfg.dynamicSmemBytes = sizeof(uint4) * 2 * D_BATCH * DT;
   cfg.stream = (cudaStream_t)c.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
