@@ -334,6 +334,10 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
         }
       }
     };
+    const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
+    const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
+    const bool lin = lloc >= 0 && lloc < a.Vl;
+    const float zl = lin ? d_load(z + lloc) : 0.f;
     int stage = 0;
     for (int k = 0; k < full; ++k, stage = STAGE - stage) {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -342,10 +346,6 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     }
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     if (left > 0) batch(stage, left);
-    const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
-    const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
-    const bool lin = lloc >= 0 && lloc < a.Vl;
-    const float zl = lin ? d_load(z + lloc) : 0.f;
     float s1, st;
     acc.finish(c1, ct, s1, st);
     // elements one by one: before the first and behind the last vector
@@ -645,11 +645,12 @@ static int d_mode(const DistillCall& c) {
   if (c.labels == 0 || c.tau == 1.) return D_ONE;
   return c.tau == 2. ? D_SQUARE : c.tau == 4. ? D_FOURTH : D_TWO;
 }
-// Threads of a CTA: two batches of loads each, as far as 64 to 256 threads give that.  A row has some microseconds of its own (the
-// entries, two rounds of reductions), so short rows take small CTAs and the SM holds more of them.
+// Threads of a CTA: four batches of loads each, as far as 32 to 256 threads give that.  A row has some microseconds of its own (the
+// entries, two rounds of reductions), so short rows take small CTAs and the SM holds more of them.  Forward / backward with 256, 64 and 32
+// threads at 16384 x 4000: 160 / 172, 66 / 76 and 54 / 68 us; with 128 and 64 at 16384 x 8000: 91 / 113 and 76 / 109 us.
 static int d_threads(const DistillCall& c, int per_vec) {
   const int64_t vecs = c.Vl / per_vec;
-  return vecs >= 8 * 256 ? 256 : vecs >= 8 * 128 ? 128 : 64;
+  return vecs >= 16 * 256 ? 256 : vecs >= 16 * 128 ? 128 : vecs >= 16 * 64 ? 64 : 32;
 }
 // CTAs that share a row: where there are fewer rows than the GPU holds CTAs, as long as each thread still has a vector.
 static int d_parts(const DistillCall& c, int threads, int per_vec, int most) {
@@ -690,7 +691,8 @@ template <typename T>
 static cudaError_t d_launch_fwd(const DistillCall& c, float* ce, float* kd, float4* saved, float4* stats) {
   const int threads = d_threads(c, DVec<T>::N);
   if (threads == 256) return d_launch_fwd_as<T, 256>(c, ce, kd, saved, stats);
-  return threads == 128 ? d_launch_fwd_as<T, 128>(c, ce, kd, saved, stats) : d_launch_fwd_as<T, 64>(c, ce, kd, saved, stats);
+  if (threads == 128) return d_launch_fwd_as<T, 128>(c, ce, kd, saved, stats);
+  return threads == 64 ? d_launch_fwd_as<T, 64>(c, ce, kd, saved, stats) : d_launch_fwd_as<T, 32>(c, ce, kd, saved, stats);
 }
 template <typename T, int DT>
 static void d_launch_bwd_as(const DistillCall& c, const float4* saved, const float* g_ce, const float* g_kd, void* out, int64_t out_ld) {
@@ -707,7 +709,8 @@ static void d_launch_bwd(const DistillCall& c, const float4* saved, const float*
   const int threads = d_threads(c, DVec<T>::N);
   if (threads == 256) d_launch_bwd_as<T, 256>(c, saved, g_ce, g_kd, out, out_ld);
   else if (threads == 128) d_launch_bwd_as<T, 128>(c, saved, g_ce, g_kd, out, out_ld);
-  else d_launch_bwd_as<T, 64>(c, saved, g_ce, g_kd, out, out_ld);
+  else if (threads == 64) d_launch_bwd_as<T, 64>(c, saved, g_ce, g_kd, out, out_ld);
+  else d_launch_bwd_as<T, 32>(c, saved, g_ce, g_kd, out, out_ld);
 }
 
 }  // namespace dh
