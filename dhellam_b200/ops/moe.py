@@ -9,6 +9,7 @@ the expert GEMMs (dropless routing has data-dependent shapes).
 """
 from __future__ import annotations
 
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 from dataclasses import dataclass
 from typing import List, NamedTuple, Optional
@@ -58,9 +59,20 @@ def _router_operands(what, probs, topi, mask):
 
 def _on_kernel(probs, topi, *others):
     """Whether the kernels of csrc/balance.cu take these operands.  Both functions were composed of PyTorch ops before and still are for
-    what only those handle: CPU tensors, the library backend, tensors that are differentiated, traced or on another device."""
-    return K.use_native(probs) and probs.shape[1] <= 1024 and K.is_plain(probs) and (probs.stride(1) == 1 or probs.shape[1] == 1) \
-        and all(t is None or (t.get_device() == probs.get_device() and K.is_plain(t)) for t in (topi, *others))
+    what only those handle: CPU tensors, the library backend, tensors that are differentiated, traced or on another device, more than
+    1024 experts or 32 choices."""
+    return K.use_native(probs) and probs.shape[1] <= 1024 and topi.shape[1] <= 32 and (probs.stride(1) == 1 or probs.shape[1] == 1) \
+        and K.are_plain(probs, topi, *others)
+
+
+# The operands that both kernels share, as one block of 8-byte fields (BalCall in csrc/balance.cu): ctypes converts argument by argument.
+_ROUTER_CALL = struct.Struct("=11q")
+
+
+def _router_call(probs, topi, mask, sm_budget):
+    T, E = probs.shape
+    return _ROUTER_CALL.pack(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), topi.dtype == torch.int64, K.ptr(mask), T, E,
+                             topi.shape[1], sm_budget, K.current_raw_stream())
 
 
 def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
@@ -79,15 +91,14 @@ def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
             topi = topi.contiguous()
         if mask is not None and not mask.is_contiguous():
             mask = mask.contiguous()
-        parts = K.proto("dh_balance_parts", [c_int, c_int, c_int])(T, E, sm_budget)
-        out = torch.empty(1 + 2 * E, dtype=torch.float32, device=probs.device)
-        loss, coef, counts = out[0], out[1:1 + E], out[1 + E:].view(torch.int32)
-        scratch = torch.empty(parts * (2 * E + 1), dtype=torch.float32, device=probs.device)
+        call = _router_call(probs, topi, mask, sm_budget)
+        out = probs.new_empty(2 * E + 1)
+        coef, loss, counts = out[:E], out[E], out[E + 1:].view(torch.int32)
+        words = K.proto("dh_balance_scratch", [c_void_p], c_int64)(call)
+        scratch = probs.new_empty(words) if words else None
         base = out.data_ptr()
-        fn = K.proto("dh_balance_fwd", [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
-                                        c_void_p, c_void_p, c_void_p, c_void_p])
-        K.check(fn(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), int(topi.dtype == torch.int64), K.ptr(mask), T, E, k,
-                   scratch.data_ptr(), parts, base, base + 4 * (1 + E), base + 4, K.stream_ptr()), "dh_balance_fwd")
+        fn = K.proto("dh_balance_fwd", [c_void_p] * 5)
+        K.check(fn(call, K.ptr(scratch), base + 4 * E, base + 4 * (E + 1), base), "dh_balance_fwd")
         return loss, counts, Balance(coef, mask)
     counted = torch.ones(T, dtype=torch.bool, device=probs.device) if mask is None else mask != 0
     n = counted.sum().clamp_min(1)
@@ -124,12 +135,10 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
         if aux_scale and balance is None:
             balance = balance_loss_fwd(probs, topi)[2]
         topi, gates, d_gates = (t if t.stride(1) == 1 else t.contiguous() for t in (topi, gates, d_gates))
-        out = torch.empty((T, E), dtype=torch.float32, device=probs.device)
-        fn = K.proto("dh_router_bwd", [c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
-                                       c_float, c_void_p, c_int, c_int, c_int, c_int, c_void_p])
-        K.check(fn(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), int(topi.dtype == torch.int64), K.ptr(mask),
-                   gates.data_ptr(), gates.stride(0), d_gates.data_ptr(), d_gates.stride(0), balance.coef.data_ptr() if aux_scale else 0,
-                   aux_scale, out.data_ptr(), T, E, k, sm_budget, K.stream_ptr()), "dh_router_bwd")
+        out = probs.new_empty((T, E))
+        fn = K.proto("dh_router_bwd", [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p])
+        K.check(fn(_router_call(probs, topi, mask, sm_budget), gates.data_ptr(), gates.stride(0), d_gates.data_ptr(), d_gates.stride(0),
+                   balance.coef.data_ptr() if aux_scale else 0, aux_scale, out.data_ptr()), "dh_router_bwd")
         return out
     valid = (topi >= 0) & (topi < E)
     at = torch.where(valid, topi, torch.zeros_like(topi)).long()
