@@ -17,11 +17,11 @@
 
 namespace dh {
 
-constexpr int BT = 256;              // threads per CTA
+constexpr int BT = 256;              // threads per CTA of the backward
 constexpr int B_CLUSTER = 8;
 constexpr int B_MAX_E = 1024;
 constexpr int B_MAX_K = 32;
-constexpr int B_ROWS = 4;            // rows of a thread's column in flight
+constexpr int B_ROWS = 8;            // rows of a thread's column in flight
 
 struct BalArgs {
   const float* probs;
@@ -41,6 +41,12 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
 }
 
+__device__ __forceinline__ float bal_warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
 template <int W> struct BalVec { float v[W]; };
 template <int W>
 __device__ __forceinline__ BalVec<W> bal_load(const float* p) {
@@ -57,32 +63,33 @@ __device__ __forceinline__ BalVec<W> bal_load(const float* p) {
 // Sums of the probabilities and counts of the choices over a share of the tokens.  A CTA's threads stand for columns of W experts and,
 // as far as that leaves threads over, for several rows; a cluster joins what its CTAs have, each CTA a share of the experts.  One cluster
 // finishes by itself, several leave psum [clusters, E] and pcount [clusters, E + 1] (last: counted tokens) for the kernel below.
-template <int W>
-__global__ void __launch_bounds__(BT) balance_kernel(const BalArgs a, float* __restrict__ psum, int* __restrict__ pcount, float* __restrict__ loss,
+template <int W, int BF>
+__global__ void __launch_bounds__(BF, 1024 / BF) balance_kernel(const BalArgs a, float* __restrict__ psum, int* __restrict__ pcount, float* __restrict__ loss,
                                                      int* __restrict__ counts, float* __restrict__ coef) {
   __shared__ int cnt[B_MAX_E + 1];
   __shared__ float csum[B_MAX_E];
-  __shared__ float part[8 * 32 * 4];
+  __shared__ float part[BF * W];
   __shared__ float losses[B_CLUSTER];
-  __shared__ float red[BT / 32];
+  __shared__ float red[BF / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (int e = threadIdx.x; e <= a.E; e += BT) cnt[e] = 0;
+  for (int e = threadIdx.x; e <= a.E; e += BF) cnt[e] = 0;
   __syncthreads();
   const int64_t t0 = (int64_t)a.T * blockIdx.x / gridDim.x, t1 = (int64_t)a.T * (blockIdx.x + 1) / gridDim.x;
   const int n = (int)(t1 - t0);
-  for (int i = threadIdx.x; i < n * a.k; i += BT) {
-    const int r = i / a.k, j = i - r * a.k;
-    const int e = bal_id(a, t0 + r, j);
-    if (a.mask == nullptr || a.mask[t0 + r]) {
+  for (int r = threadIdx.x; r < n; r += BF) {
+    if (a.mask != nullptr && !a.mask[t0 + r]) continue;
+    atomicAdd(&cnt[a.E], 1);
+#pragma unroll 4
+    for (int j = 0; j < a.k; ++j) {
+      const int e = bal_id(a, t0 + r, j);
       if (e >= 0) atomicAdd(&cnt[e], 1);
-      if (j == 0) atomicAdd(&cnt[a.E], 1);
     }
   }
-  // columns: the next power of two of E / W, at most BT
+  // columns: the next power of two of E / W, at most BF
   const int groups = (a.E + W - 1) / W;
   int cols = 1;
-  while (cols < groups && cols < BT) cols <<= 1;
-  const int c = threadIdx.x & (cols - 1), r0 = threadIdx.x / cols, rows = BT / cols;
+  while (cols < groups && cols < BF) cols <<= 1;
+  const int c = threadIdx.x & (cols - 1), r0 = threadIdx.x / cols, rows = BF / cols;
   for (int first = 0; first < groups; first += cols) {
     const int g = first + c;
     float s[W];
@@ -115,20 +122,21 @@ __global__ void __launch_bounds__(BT) balance_kernel(const BalArgs a, float* __r
 #pragma unroll
       for (int q = 0; q < W; ++q) s[q] += __shfl_xor_sync(0xffffffffu, s[q], o);
     }
-    const int parts = cols < 32 ? BT / 32 : rows, mine = cols < 32 ? warp : r0;
+    const int parts = cols < 32 ? BF / 32 : rows, mine = cols < 32 ? warp : r0;
     __syncthreads();
     if (cols >= 32 || lane < cols) {
 #pragma unroll
       for (int q = 0; q < W; ++q) part[(mine * cols + c) * W + q] = s[q];
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < cols * W; e += BT) {
+    for (int e = threadIdx.x; e < cols * W; e += BF) {
       if (first * W + e >= a.E) continue;
       float t = part[e];
       for (int q = 1; q < parts; ++q) t += part[q * cols * W + e];
       csum[first * W + e] = t;
     }
   }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");       // the kernel below may be put in place
   __syncthreads();
   cluster_sync_all();
   const int me = (int)cluster_ctarank(), cluster = blockIdx.x / B_CLUSTER;
@@ -138,7 +146,7 @@ __global__ void __launch_bounds__(BT) balance_kernel(const BalArgs a, float* __r
   for (int r = 0; r < B_CLUSTER; ++r) counted += (int)ld_cluster_u32(bal_at(&cnt[a.E], r));
   const float inv = counted > 0 ? 1.f / (float)counted : 0.f;
   float l = 0.f;
-  for (int e = me + (int)threadIdx.x * B_CLUSTER; e < a.E; e += B_CLUSTER * BT) {
+  for (int e = me + (int)threadIdx.x * B_CLUSTER; e < a.E; e += B_CLUSTER * BF) {
     float s = 0.f;
     int n_e = 0;
 #pragma unroll
@@ -159,12 +167,11 @@ __global__ void __launch_bounds__(BT) balance_kernel(const BalArgs a, float* __r
   if (!alone) {
     if (me == 0 && threadIdx.x == 0) pcount[(size_t)cluster * (a.E + 1) + a.E] = counted;
   } else {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    l = bal_warp_sum(l);
     if (lane == 0) red[warp] = l;
     __syncthreads();
     if (threadIdx.x == 0) {
-      for (int q = 1; q < BT / 32; ++q) l += red[q];
+      for (int q = 1; q < BF / 32; ++q) l += red[q];
       st_cluster_f32(bal_at(&losses[me], 0), l);
     }
   }
@@ -177,34 +184,50 @@ __global__ void __launch_bounds__(BT) balance_kernel(const BalArgs a, float* __r
   }
 }
 
+// What the clusters have: 1024 threads, as many of them for an expert as that leaves.
 __global__ void __launch_bounds__(1024) balance_finish_kernel(const float* __restrict__ psum, const int* __restrict__ pcount, int parts, int E, int k,
                                                               float* __restrict__ loss, int* __restrict__ counts, float* __restrict__ coef) {
+  __shared__ float sums[1024];
+  __shared__ int cnts[1024];
   __shared__ float red[32];
-  int n = 0;
-  for (int p = threadIdx.x & 31; p < parts; p += 32) n += pcount[(size_t)p * (E + 1) + E];
-  n = __reduce_add_sync(0xffffffffu, n);
-  const float inv = n > 0 ? 1.f / (float)n : 0.f;
+  __shared__ int counted;
+  if (threadIdx.x == 0) counted = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if ((int)threadIdx.x < parts) atomicAdd(&counted, pcount[(size_t)threadIdx.x * (E + 1) + E]);
+  int cols = 32;
+  while (cols < E) cols <<= 1;
+  const int e = threadIdx.x & (cols - 1), step = 1024 / cols;
+  float s = 0.f;
+  int c = 0;
+  if (e < E) {
+#pragma unroll 8
+    for (int p = threadIdx.x / cols; p < parts; p += step) {
+      s += psum[(size_t)p * E + e];
+      c += pcount[(size_t)p * (E + 1) + e];
+    }
+  }
+  sums[threadIdx.x] = s;
+  cnts[threadIdx.x] = c;
+  __syncthreads();
   float l = 0.f;
   if ((int)threadIdx.x < E) {
-    float s = 0.f;
-    int c = 0;
-#pragma unroll 4
-    for (int p = 0; p < parts; ++p) {
-      s += psum[(size_t)p * E + threadIdx.x];
-      c += pcount[(size_t)p * (E + 1) + threadIdx.x];
+    for (int q = 1; q < step; ++q) {
+      s += sums[q * cols + e];
+      c += cnts[q * cols + e];
     }
+    const float inv = counted > 0 ? 1.f / (float)counted : 0.f;
     const float w = (float)c * inv * inv * ((float)E / (float)k);
-    counts[threadIdx.x] = c;
-    coef[threadIdx.x] = w;
+    counts[e] = c;
+    coef[e] = w;
     l = w * s;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  l = bal_warp_sum(l);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = l;
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) l += red[w];
-    *loss = l;
+  if (threadIdx.x < 32) {
+    l = bal_warp_sum(red[threadIdx.x]);
+    if (threadIdx.x == 0) *loss = l;
   }
 }
 
@@ -213,15 +236,23 @@ struct RouterArgs {
   float* out;
   int64_t g_stride, dg_stride;
   float weight;
-  int lanes;                                 // threads of a row: a power of two, at least k
 };
 
-// `lanes` threads per token, each with NV vectors of W experts; thread j of them also has the j-th choice.  The row is written with the
-// balance term alone and its k chosen experts once more behind that (the few that were chosen need no search by the others).
-template <int W, int NV>
+template <int L>
+__device__ __forceinline__ void bal_group_sum(float& a, float& b) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, o);
+    b += __shfl_xor_sync(0xffffffffu, b, o);
+  }
+}
+
+// L threads per token (a power of two, at least k), each with NV vectors of W experts; thread j of them also has the j-th choice.  The row
+// is written with the balance term alone and its k chosen experts once more behind that (no search for the few that were chosen).
+template <int W, int L, int NV>
 __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const RouterArgs b) {
-  const int lane = threadIdx.x & 31, L = b.lanes, l = lane & (L - 1);
-  const int per_warp = 32 / L;
+  const int lane = threadIdx.x & 31, l = lane & (L - 1);
+  constexpr int PER_WARP = 32 / L;
   float co[NV][W];
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -230,8 +261,8 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
       const int e = (i * L + l) * W + q;
       co[i][q] = b.coef != nullptr && e < a.E ? b.weight * b.coef[e] : 0.f;
     }
-  const int64_t step = (int64_t)gridDim.x * (BT / 32) * per_warp;
-  for (int64_t base = ((int64_t)blockIdx.x * (BT / 32) + (threadIdx.x >> 5)) * per_warp; base < a.T; base += step) {
+  const int step = gridDim.x * (BT / 32) * PER_WARP;
+  for (int base = (blockIdx.x * (BT / 32) + (threadIdx.x >> 5)) * PER_WARP; base < a.T; base += step) {
     const int64_t t = base + lane / L;
     const bool row = t < a.T;
     const float* p = a.probs + (row ? t : 0) * a.p_stride;
@@ -244,29 +275,25 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
       if (row && e < a.E) v[i] = bal_load<W>(p + e);
     }
     int id = -1;
-    float dg = 0.f, g = 0.f, pj = 0.f;
+    float dot = 0.f, dg = 0.f, pj = 0.f;
     if (row && l < a.k) {
       id = bal_id(a, t, l);
       dg = b.d_gates[t * b.dg_stride + l];
-      g = b.gates[t * b.g_stride + l];
+      const float g = b.gates[t * b.g_stride + l];
+      if (id >= 0) { pj = p[id]; dot = dg * g; }
     }
     const bool counts = row && (a.mask == nullptr || a.mask[t] != 0);
-    if (id >= 0) pj = p[id];
-    float dot = id >= 0 ? dg * g : 0.f, sel = pj;
-    for (int o = L >> 1; o > 0; o >>= 1) {
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-      sel += __shfl_xor_sync(0xffffffffu, sel, o);
-    }
+    float sel = pj;
+    bal_group_sum<L>(dot, sel);
     float u = id >= 0 && sel != 0.f ? (dg - dot) / sel : 0.f;
-    float all = u * pj;
+    float all = u * pj, bal = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
-      for (int q = 0; q < W; ++q) {
-        const int e = (i * L + l) * W + q;
-        if (counts && e < a.E) all += co[i][q] * v[i].v[q];
-      }
-    for (int o = L >> 1; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+      for (int q = 0; q < W; ++q) bal = fmaf(co[i][q], v[i].v[q], bal);
+    bal_group_sum<L>(all, bal);
+    if (counts) all += bal;
+    const float on = counts ? 1.f : 0.f;
     float* o = b.out + (row ? t : 0) * a.E;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -274,22 +301,29 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
       if (!row || e >= a.E) continue;
       float r[W];
 #pragma unroll
-      for (int q = 0; q < W; ++q) r[q] = v[i].v[q] * ((counts ? co[i][q] : 0.f) - all);
+      for (int q = 0; q < W; ++q) r[q] = v[i].v[q] * fmaf(co[i][q], on, -all);
       if constexpr (W == 4) *reinterpret_cast<float4*>(o + e) = make_float4(r[0], r[1], r[2], r[3]);
       else o[e] = r[0];
     }
     // an expert that was chosen twice gets both choices' gradients, in the order of the choices
-    const unsigned int twins = __match_any_sync(0xffffffffu, id >= 0 ? (lane / L) * B_MAX_E + id : -1 - lane);
-    if (__any_sync(0xffffffffu, (twins & (twins - 1)) != 0)) {
+    bool twice = false;
+#pragma unroll
+    for (int q = 1; q <= L / 2; ++q) {
+      const int other = __shfl_sync(0xffffffffu, id, (l + q) & (L - 1), L);
+      twice |= id >= 0 && other == id;
+    }
+    if (__any_sync(0xffffffffu, twice)) {
       float sum = 0.f;
-      for (int q = 0; q < 32; ++q) {
-        const float other = __shfl_sync(0xffffffffu, u, q);
-        if (twins >> q & 1) sum += other;
+#pragma unroll 1
+      for (int q = 0; q < L; ++q) {
+        const float x = __shfl_sync(0xffffffffu, u, q, L);
+        const int other = __shfl_sync(0xffffffffu, id, q, L);
+        if (other == id) sum += x;
       }
       u = sum;
     }
     __syncwarp();
-    if (id >= 0) o[id] = pj * ((counts && b.coef != nullptr ? b.weight * b.coef[id] : 0.f) - all + u);
+    if (id >= 0) o[id] = pj * (fmaf(b.coef != nullptr ? b.weight * b.coef[id] : 0.f, on, -all) + u);
     __syncwarp();
   }
 }
@@ -318,27 +352,47 @@ static int bal_budget(const BalCall& c) {
   return (c.budget <= 0 || c.budget > sms) ? sms : (int)c.budget;
 }
 static bool bal_wide(const BalCall& c) { return c.E % 4 == 0 && c.p_stride % 4 == 0 && (c.probs & 15) == 0; }
-// Clusters of the forward: one (a single launch) up to B_ALONE probabilities, beyond it up to two CTAs per SM.
+// Clusters of the forward: one (a single launch) up to B_ALONE probabilities, beyond it two CTAs of 256 threads per SM (65536 x 256: 21 us,
+// with four of them 25, with one of 1024 threads 34).  A budget of fewer SMs than a cluster's CTAs still takes one cluster.
 constexpr int64_t B_ALONE = 1 << 19;
 static int bal_clusters(const BalCall& c) {
   if (c.T * c.E <= B_ALONE) return 1;
-  const int64_t want = c.T * c.E / (1 << 16) / B_CLUSTER, most = 2 * bal_budget(c) / B_CLUSTER;
+  const int64_t want = c.T * c.E / (1 << 14) / B_CLUSTER, most = 2 * bal_budget(c) / B_CLUSTER;
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
 
-template <int W>
-static void router_launch(const BalCall& c, const RouterArgs& r, int vecs, cudaStream_t s) {
-  const int64_t warps = (c.T + 32 / r.lanes - 1) / (32 / r.lanes), blocks = (warps + BT / 32 - 1) / (BT / 32);
-  const int64_t most = 8ll * bal_budget(c);
-  const unsigned int grid = (unsigned int)(blocks < most ? blocks : most);
-  const BalArgs a = bal_args(c);
-  if (vecs <= 1) router_bwd_kernel<W, 1><<<grid, BT, 0, s>>>(a, r);
-  else if (vecs <= 2) router_bwd_kernel<W, 2><<<grid, BT, 0, s>>>(a, r);
-  else if (vecs <= 4) router_bwd_kernel<W, 4><<<grid, BT, 0, s>>>(a, r);
-  else if (vecs <= 8) router_bwd_kernel<W, 8><<<grid, BT, 0, s>>>(a, r);
-  else if (W == 1 && vecs <= 16) router_bwd_kernel<W, W == 1 ? 16 : 1><<<grid, BT, 0, s>>>(a, r);
-  else router_bwd_kernel<W, W == 1 ? 32 : 1><<<grid, BT, 0, s>>>(a, r);
+template <int W, int L, int NV>
+static void router_launch(const BalCall& c, const RouterArgs& r) {
+  const int64_t warps = (c.T + 32 / L - 1) / (32 / L), blocks = (warps + BT / 32 - 1) / (BT / 32), most = 8ll * bal_budget(c);
+  router_bwd_kernel<W, L, NV><<<(unsigned int)(blocks < most ? blocks : most), BT, 0, (cudaStream_t)c.stream>>>(bal_args(c), r);
+}
+// Vectors of a thread: up to MOST of them.
+template <int W, int L, int MOST>
+static void router_launch_lanes(const BalCall& c, const RouterArgs& r, int vecs) {
+  if (vecs <= 1) router_launch<W, L, 1>(c, r);
+  else if (vecs <= 2) router_launch<W, L, 2>(c, r);
+  else if (vecs <= 4) router_launch<W, L, 4>(c, r);
+  else if (MOST <= 8 || vecs <= 8) router_launch<W, L, MOST < 8 ? MOST : 8>(c, r);
+  else if (MOST <= 16 || vecs <= 16) router_launch<W, L, MOST < 16 ? MOST : 16>(c, r);
+  else router_launch<W, L, MOST>(c, r);
+}
+// Threads of a token: as few as hold its row in MOST vectors each and have a choice each; 32 with up to LAST vectors where MOST are too few.
+// MOST: 65536 x 256 with vectors of four 46, 32 and 37 us for 2, 4 and 8 of them, 65536 x 255 one by one 55 and 33 us for 8 and 16.
+template <int W, int MOST, int LAST>
+static void router_launch_wide(const BalCall& c, const RouterArgs& r) {
+  const int groups = (int)((c.E + W - 1) / W);
+  int lanes = 1;
+  while (lanes < 32 && (lanes * MOST < groups || lanes < c.k)) lanes *= 2;
+  const int vecs = (groups + lanes - 1) / lanes;
+  switch (lanes) {
+    case 1: return router_launch_lanes<W, 1, MOST>(c, r, vecs);
+    case 2: return router_launch_lanes<W, 2, MOST>(c, r, vecs);
+    case 4: return router_launch_lanes<W, 4, MOST>(c, r, vecs);
+    case 8: return router_launch_lanes<W, 8, MOST>(c, r, vecs);
+    case 16: return router_launch_lanes<W, 16, MOST>(c, r, vecs);
+    default: return router_launch_lanes<W, 32, LAST>(c, r, vecs);
+  }
 }
 
 }  // namespace dh
@@ -364,9 +418,12 @@ int dh_balance_fwd(const void* call, void* scratch, void* loss, void* counts, vo
   }
   float* psum = (float*)scratch;
   int* pcount = n > 1 ? (int*)(psum + (size_t)n * c.E) : nullptr;
+  // one cluster alone asks for everything itself: with 256 threads each its CTAs took 24 us for 5003 x 61, with 1024 14
+  void (*const kernels[2][2])(const BalArgs, float*, int*, float*, int*, float*) = {{balance_kernel<1, 1024>, balance_kernel<4, 1024>},
+                                                                                   {balance_kernel<1, 256>, balance_kernel<4, 256>}};
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n * B_CLUSTER);
-  cfg.blockDim = dim3(BT);
+  cfg.blockDim = dim3(n > 1 ? 256 : 1024);
   cfg.stream = (cudaStream_t)c.stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -374,10 +431,15 @@ int dh_balance_fwd(const void* call, void* scratch, void* loss, void* counts, vo
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = bal_wide(c) ? cudaLaunchKernelEx(&cfg, balance_kernel<4>, bal_args(c), psum, pcount, (float*)loss, (int*)counts, (float*)coef)
-                                    : cudaLaunchKernelEx(&cfg, balance_kernel<1>, bal_args(c), psum, pcount, (float*)loss, (int*)counts, (float*)coef);
-  if (e == cudaSuccess && n > 1)
-    balance_finish_kernel<<<1, 1024, 0, cfg.stream>>>(psum, pcount, n, (int)c.E, (int)c.k, (float*)loss, (int*)counts, (float*)coef);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernels[n > 1][bal_wide(c)], bal_args(c), psum, pcount, (float*)loss, (int*)counts, (float*)coef);
+  if (e == cudaSuccess && n > 1) {
+    cfg.gridDim = dim3(1);
+    cfg.blockDim = dim3(1024);
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    e = cudaLaunchKernelEx(&cfg, balance_finish_kernel, (const float*)psum, (const int*)pcount, n, (int)c.E, (int)c.k, (float*)loss, (int*)counts,
+                           (float*)coef);
+  }
   return bal_rc("dh_balance_fwd", e);
 }
 // out [T, E] fp32 contiguous, 16-byte aligned.  coef may be null (no balance term).
@@ -386,13 +448,9 @@ int dh_router_bwd(const void* call, const void* gates, int64_t g_stride, const v
   const BalCall& c = *(const BalCall*)call;
   if (int rc = bal_refuse("dh_router_bwd", c)) return rc;
   if (c.T == 0) return 0;
-  RouterArgs r{(const float*)gates, (const float*)d_gates, (const float*)coef, (float*)out, g_stride, dg_stride, weight, 1};
-  const bool wide = bal_wide(c) && ((uintptr_t)out & 15) == 0;
-  const int groups = (int)(wide ? c.E / 4 : c.E);
-  while (r.lanes < 32 && (r.lanes < groups || r.lanes < c.k)) r.lanes *= 2;
-  const int vecs = (groups + r.lanes - 1) / r.lanes;
-  if (wide) router_launch<4>(c, r, vecs, (cudaStream_t)c.stream);
-  else router_launch<1>(c, r, vecs, (cudaStream_t)c.stream);
+  const RouterArgs r{(const float*)gates, (const float*)d_gates, (const float*)coef, (float*)out, g_stride, dg_stride, weight};
+  if (bal_wide(c) && ((uintptr_t)out & 15) == 0) router_launch_wide<4, 4, 8>(c, r);
+  else router_launch_wide<1, 16, 32>(c, r);
   return bal_rc("dh_router_bwd", cudaSuccess);
 }
 

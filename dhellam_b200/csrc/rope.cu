@@ -143,6 +143,13 @@ __global__ void __launch_bounds__(RT) rope_heads_kernel(const RopeArgs a) {
   }
 }
 
+// All fields 8 bytes wide, as the Python layer packs them.  ptrs: q in, q out, k in, k out; strides (elements): for each of them the outer
+// row, inner row and head stride; rows are outer x inner.
+struct RopeCall {
+  int64_t ptrs[4], strides[12], heads_q, heads_k, pos, pos64, freq, rows, inner, d, rotated, interleaved, f32, transposed, budget, stream;
+  double scale;
+};
+
 template <typename T, int V>
 static void rope_launch(const RopeArgs& a, int interleaved, int grid, cudaStream_t s) {
   if (interleaved) rope_heads_kernel<T, V, true><<<grid, RT, 0, s>>>(a);
@@ -155,25 +162,27 @@ using namespace dh;
 
 extern "C" {
 
-// Rotates the heads of q (and of k, unless heads_k is 0).  ptrs: q in, q out, k in, k out; strides (elements): for each of
-// q in, q out, k in, k out the outer row, inner row and head stride; rows are outer x inner with `inner` rows in the second dimension.
-// f32: 0 bf16, 1 fp32.  in == out (with equal strides) works in place.
-int dh_rope_heads(void* const* ptrs, const int64_t* strides, int heads_q, int heads_k, const void* pos, int pos64, const void* freq, int64_t rows,
-                  int64_t inner, int d, int rotated, int interleaved, int f32, float scale, int transposed, int sm_budget, cudaStream_t s) {
-  if (heads_q < 0 || heads_k < 0 || d <= 0 || d > 65536 || rotated <= 0 || rotated > d || (rotated & 1) || rows < 0 || inner <= 0 || inner > INT32_MAX) {
+// Rotates the heads of q (and of k, unless heads_k is 0); in == out (with equal strides) works in place.
+int dh_rope_heads(const void* call) {
+  const RopeCall& c = *(const RopeCall*)call;
+  const int64_t rows = c.rows, inner = c.inner;
+  const int heads_q = (int)c.heads_q, heads_k = (int)c.heads_k, d = (int)c.d, rotated = (int)c.rotated;
+  const int64_t* ptrs = c.ptrs;
+  if (c.heads_q < 0 || c.heads_k < 0 || c.heads_q + c.heads_k > INT32_MAX || c.d <= 0 || c.d > 65536 || c.rotated <= 0 || c.rotated > c.d ||
+      (c.rotated & 1) || rows < 0 || inner <= 0 || inner > INT32_MAX) {
     set_last_error_c("dh_rope_heads", "sizes out of range (an even number of rotated elements, at most the head size)");
     return (int)cudaErrorInvalidValue;
   }
   if (rows == 0 || heads_q + heads_k == 0) return 0;
-  const int size = f32 ? 4 : 2;
+  const int size = c.f32 ? 4 : 2;
   const bool in_place = (heads_q == 0 || ptrs[0] == ptrs[1]) && (heads_k == 0 || ptrs[2] == ptrs[3]);
   // the widest vector that divides half the rotated part, the rest, every address and every stride
   uint64_t odd = (uint64_t)(rotated / 2) * size;
   if (!in_place) odd |= (uint64_t)(d - rotated) * size;
   for (int i = 0; i < 4; ++i) {
     if ((i < 2 ? heads_q : heads_k) == 0) continue;
-    odd |= (uint64_t)(uintptr_t)ptrs[i];
-    for (int j = 0; j < 3; ++j) odd |= (uint64_t)(strides[3 * i + j] * size);
+    odd |= (uint64_t)ptrs[i];
+    for (int j = 0; j < 3; ++j) odd |= (uint64_t)(c.strides[3 * i + j] * size);
   }
   const int bytes = (odd & 15) == 0 ? 16 : (odd & 7) == 0 ? 8 : (odd & 3) == 0 ? 4 : 2;
   const int V = bytes / size;
@@ -183,23 +192,25 @@ int dh_rope_heads(void* const* ptrs, const int64_t* strides, int heads_q, int he
   }
   RopeArgs a;
   for (int i = 0; i < 2; ++i) {
-    const int64_t* st = strides + 6 * i;
-    a.t[i] = RopeTensor{ptrs[2 * i], ptrs[2 * i + 1], st[0], st[1], st[2], st[3], st[4], st[5]};
+    const int64_t* st = c.strides + 6 * i;
+    a.t[i] = RopeTensor{(const void*)ptrs[2 * i], (void*)ptrs[2 * i + 1], st[0], st[1], st[2], st[3], st[4], st[5]};
   }
   a.heads[0] = heads_q;
   a.heads[1] = heads_k;
-  a.pos = pos;
-  a.freq = (const double*)freq;
-  a.scale = scale;
-  a.sign = transposed ? -1.f : 1.f;
-  a.pos64 = pos64;
+  a.pos = (const void*)c.pos;
+  a.freq = (const double*)c.freq;
+  a.scale = (float)c.scale;
+  a.sign = c.transposed ? -1.f : 1.f;
+  a.pos64 = (int)c.pos64;
   a.inner = (int)inner;
   a.half = rotated / 2;
   a.d = d;
   a.rot_units = a.half / V;
   a.units = a.rot_units + (in_place ? 0 : (d - rotated + 2 * V - 1) / (2 * V));
   const int sms = dh_sm_count();
-  const int budget = (sm_budget <= 0 || sm_budget > sms) ? sms : sm_budget;
+  const int budget = (c.budget <= 0 || c.budget > sms) ? sms : (int)c.budget;
+  const int interleaved = (int)c.interleaved;
+  const cudaStream_t s = (cudaStream_t)c.stream;
   // threads that share the heads of a row: enough of them to fill half of the GPU's threads, where there are that few rows
   a.groups = 1;
   while (a.groups * 2 <= heads_q + heads_k && rows * a.units * a.groups < (int64_t)budget * 1024) a.groups *= 2;
@@ -209,7 +220,7 @@ int dh_rope_heads(void* const* ptrs, const int64_t* strides, int heads_q, int he
     a.rows = rows - r < most ? rows - r : most;
     const int64_t blocks = (a.rows * a.units * a.groups + RT - 1) / RT;
     const int grid = (int)(blocks < (int64_t)budget * 8 ? blocks : (int64_t)budget * 8);
-    if (f32) {
+    if (c.f32) {
       if (V == 4) rope_launch<float, 4>(a, interleaved, grid, s);
       else if (V == 2) rope_launch<float, 2>(a, interleaved, grid, s);
       else rope_launch<float, 1>(a, interleaved, grid, s);

@@ -12,7 +12,8 @@ needed for the Llama family.  Two forms:
 from __future__ import annotations
 
 import math
-from ctypes import c_float, c_int, c_int64, c_void_p
+import struct
+from ctypes import c_int, c_void_p
 from dataclasses import dataclass
 
 import torch
@@ -122,12 +123,40 @@ def _turn_ref(x, positions, freq, interleaved, scale, transposed):
     return y.to(x.dtype)
 
 
-def _heads_fit(x, lead, d, dtype):
+# The operands of the kernel as one block of 8-byte fields (RopeCall in csrc/rope.cu): ctypes converts argument by argument, which takes
+# several microseconds where a small call has 15 in all.
+_ROPE_CALL = struct.Struct("=30qd")
+
+
+def _fits(x, lead, d, dtype):
     return x.dim() in (3, 4) and x.shape[:-2] == lead and x.shape[-1] == d and x.dtype == dtype and (x.stride(-1) == 1 or d == 1)
 
 
+def _check(q, k, positions, freq, out, what):
+    lead, d = q.shape[:-2], q.shape[-1] if q.dim() else 0
+    if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{what}: one int32 or int64 position for each of {tuple(lead)} rows, got {positions.dtype} {tuple(positions.shape)}")
+    if freq.dtype != torch.float64 or freq.dim() != 1 or not 0 < 2 * freq.numel() <= d:
+        raise ValueError(f"{what}: fp64 frequencies of at most half of the {d} elements of a head, got {freq.dtype} {tuple(freq.shape)}")
+    inputs = (q,) if k is None else (q, k)
+    for x in inputs:
+        if not _fits(x, lead, d, q.dtype):
+            raise ValueError(f"{what}: queries and keys are [rows..., heads, {d}] of one type, with elements side by side")
+    if out is None:
+        return
+    for x, o in zip(inputs, out):
+        if o.shape != x.shape or not _fits(o, lead, d, q.dtype) or any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+            raise ValueError(f"{what}: an output has its input's shape and type, room for every row and head and elements side by side")
+        in_place = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
+        if not in_place and any(o.untyped_storage().data_ptr() == y.untyped_storage().data_ptr() for y in inputs):
+            raise ValueError(f"{what}: an output is its own input or shares no memory with the inputs")
+    if k is not None and out[0].data_ptr() == out[1].data_ptr() and q.numel() and k.numel():
+        raise ValueError(f"{what}: queries and keys have outputs of their own")
+
+
 def _strides(x):
-    return (x.stride(0), 0, x.stride(1)) if x.dim() == 3 else (x.stride(0), x.stride(1), x.stride(2))
+    s = x.stride()
+    return s[:3] if len(s) == 4 else (s[0], 0, s[1])
 
 
 def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget, stream, what):
@@ -135,46 +164,32 @@ def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
         operands = (q, k, positions, freq) + (tuple(out) if out is not None else ())
         return K.run_on_stream(stream, operands, lambda: _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
                                                                None, what))
-    lead, d = q.shape[:-2], q.shape[-1]
-    pairs = [(q, out[0] if out is not None else None)] + ([(k, out[1] if out is not None else None)] if k is not None else [])
-    if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"{what}: one int32 or int64 position for each of {tuple(lead)} rows, got {positions.dtype} {tuple(positions.shape)}")
-    if freq.dtype != torch.float64 or freq.dim() != 1 or not 0 < 2 * freq.numel() <= d:
-        raise ValueError(f"{what}: fp64 frequencies of at most half of the {d} elements of a head, got {freq.dtype} {tuple(freq.shape)}")
-    for x, o in pairs:
-        if not _heads_fit(x, lead, d, q.dtype):
-            raise ValueError(f"{what}: queries and keys are [rows..., heads, {d}] of one type, with elements side by side")
-        if o is None:
-            continue
-        if o.shape != x.shape or not _heads_fit(o, lead, d, q.dtype):
-            raise ValueError(f"{what}: an output has its input's shape and type, with elements side by side")
-        in_place = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
-        if not in_place and any(o.untyped_storage().data_ptr() == y.untyped_storage().data_ptr() for y, _ in pairs):
-            raise ValueError(f"{what}: an output is its own input or shares no memory with the inputs")
-        if any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
-            raise ValueError(f"{what}: an output has room for every row and head")
-    if out is not None and k is not None and out[0].data_ptr() == out[1].data_ptr() and q.numel() and k.numel():
-        raise ValueError(f"{what}: queries and keys have outputs of their own")
+    _check(q, k, positions, freq, out, what)
+    oq, ok = out if out is not None else (None, None)
     if not K.use_native(q):
-        res = [_turn_ref(x, positions, freq, interleaved, scale, transposed) for x, _ in pairs]
-        res = [r if o is None else o.copy_(r) for r, (_, o) in zip(res, pairs)]
-        return res[0], (res[1] if k is not None else None)
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{what}: the sm_100a kernel rotates bf16 and fp32, not {q.dtype}")
-    K.require_current_device(what, q, k, positions, freq, *(out or ()))
+        rq = _turn_ref(q, positions, freq, interleaved, scale, transposed)
+        rk = _turn_ref(k, positions, freq, interleaved, scale, transposed) if k is not None else None
+        return (rq, rk) if out is None else (oq.copy_(rq), ok.copy_(rk) if k is not None else None)
+    shape, dtype = q.shape, q.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float32:
+        raise ValueError(f"{what}: the sm_100a kernel rotates bf16 and fp32, not {dtype}")
+    K.require_current_device(what, q, k, positions, freq, oq, ok)
     if not positions.is_contiguous() or not freq.is_contiguous():
         raise ValueError(f"{what}: positions and frequencies must be contiguous")
-    pairs = [(x, torch.empty(x.shape, dtype=x.dtype, device=x.device) if o is None else o) for x, o in pairs]
-    ptrs, strides = (c_void_p * 4)(), (c_int64 * 12)()
-    for i, (x, o) in enumerate(pairs):
-        ptrs[2 * i], ptrs[2 * i + 1] = x.data_ptr(), o.data_ptr()
-        strides[6 * i:6 * i + 6] = _strides(x) + _strides(o)
-    fn = K.proto("dh_rope_heads", [c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_int, c_int,
-                                   c_float, c_int, c_int, c_void_p])
-    K.check(fn(ptrs, strides, q.shape[-2], 0 if k is None else k.shape[-2], positions.data_ptr(), int(positions.dtype == torch.int64),
-               freq.data_ptr(), positions.numel(), 1 if len(lead) == 1 else max(lead[1], 1), d, 2 * freq.numel(), int(bool(interleaved)),
-               int(q.dtype == torch.float32), scale, int(transposed), sm_budget, K.stream_ptr()), "dh_rope_heads")
-    return pairs[0][1], (pairs[1][1] if k is not None else None)
+    if oq is None:
+        oq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    if k is None:
+        ok, heads_k, keys, key_strides = None, 0, (0, 0), (0, 0, 0, 0, 0, 0)
+    else:
+        if ok is None:
+            ok = torch.empty_like(k, memory_format=torch.contiguous_format)
+        heads_k, keys, key_strides = k.shape[-2], (k.data_ptr(), ok.data_ptr()), _strides(k) + _strides(ok)
+    call = _ROPE_CALL.pack(q.data_ptr(), oq.data_ptr(), *keys, *_strides(q), *_strides(oq), *key_strides, shape[-2], heads_k,
+                           positions.data_ptr(), positions.dtype == torch.int64, freq.data_ptr(), positions.numel(),
+                           1 if len(shape) == 3 else shape[1] or 1, shape[-1], 2 * freq.numel(), bool(interleaved), dtype == torch.float32,
+                           transposed, sm_budget, K.current_raw_stream(), scale)
+    K.check(K.proto("dh_rope_heads", [c_void_p])(call), "dh_rope_heads")
+    return oq, ok
 
 
 def rope_fwd(q, k, positions, freq, interleaved: bool = False, scale: float = 1.0, out=None, sm_budget: int = 0, stream=None):
