@@ -9,8 +9,15 @@
 // turns in 64 bits and reduced to [-1/2, 1/2] before it is rounded to 32, so far positions lose nothing (a 32-bit product is off
 // by 0.03 rad at position 10^6).
 //
-// One thread holds the cosines and sines of V pairs of one row in registers and walks over heads with them: two 16-byte loads and
-// stores per head.  Bound by memory.
+// One thread holds the cosines and sines of V pairs of one row in registers and walks over heads with them, several in flight: two 16-byte
+// loads and stores per head.  Bound by memory: 65536 x 40 heads of 128, 217 us (6.2 TB/s).  A table of a CTA's angles in shared memory, so
+// that threads that share a row do not compute them anew, was slower (225 us; 65536 x 3 heads 39 against 27), and so was one head at a
+// time (243 us).
+//
+// Interleaved, a vector may hold pairs that are turned and pairs that stay, so V follows from addresses and strides alone.  In halves it has
+// to divide half the rotated elements too (16384 x 80 heads of 96, 38 rotated: 93 us interleaved, 224 us in halves, element by element).
+// Elements that are only copied stay with the pairs of their head: as work items behind all pairs they tore the lines of memory apart
+// (3799 x 80 heads of 128, 64 rotated: 37 against 51 us).
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -39,40 +46,82 @@ struct RopeArgs {
   long long row0, rows;
 };
 
+// V elements as they are loaded and stored, and as fp32.
 template <int BYTES> struct RawOf;
 template <> struct RawOf<16> { using type = uint4; };
 template <> struct RawOf<8> { using type = uint2; };
 template <> struct RawOf<4> { using type = uint32_t; };
 template <> struct RawOf<2> { using type = uint16_t; };
+template <typename T, int V> using RopeRaw = typename RawOf<sizeof(T) * V>::type;
 
 template <typename T, int V>
-struct alignas(sizeof(T) * V) RopeVec {
-  T e[V];
-};
-
-__device__ __forceinline__ float rope_f(float x) { return x; }
-__device__ __forceinline__ float rope_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <typename T> __device__ __forceinline__ T rope_t(float x);
-template <> __device__ __forceinline__ float rope_t<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 rope_t<__nv_bfloat16>(float x) { return __float2bfloat16(x); }
-
-template <typename T, int V>
-__device__ __forceinline__ RopeVec<T, V> rope_load(const T* p) {
-  using R = typename RawOf<sizeof(T) * V>::type;
-  union { R r; RopeVec<T, V> v; } u;
-  u.r = *reinterpret_cast<const R*>(p);
-  return u.v;
+__device__ __forceinline__ void rope_unpack(const RopeRaw<T, V>& r, float (&f)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) f[j] = __uint_as_float(w[j]);
+  } else if constexpr (V == 1) {
+    f[0] = __uint_as_float((uint32_t)r << 16);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) { const float2 p = unpack_bf16x2(w[j]); f[2 * j] = p.x; f[2 * j + 1] = p.y; }
+  }
 }
 template <typename T, int V>
-__device__ __forceinline__ void rope_store(T* p, const RopeVec<T, V>& v) {
-  using R = typename RawOf<sizeof(T) * V>::type;
-  union { R r; RopeVec<T, V> v; } u;
-  u.v = v;
-  *reinterpret_cast<R*>(p) = u.r;
+__device__ __forceinline__ RopeRaw<T, V> rope_pack(const float (&f)[V]) {
+  RopeRaw<T, V> r;
+  if constexpr (sizeof(T) == 4) {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V; ++j) w[j] = __float_as_uint(f[j]);
+  } else if constexpr (V == 1) {
+    r = __bfloat16_as_ushort(__float2bfloat16(f[0]));
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&r);
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) w[j] = pack_bf16x2(f[2 * j], f[2 * j + 1]);
+  }
+  return r;
+}
+// Turns V pairs: x the first, y the second elements; interleaved, x has the first V/2 pairs, y the others, and those from n on stay.
+template <typename T, int V, bool INTERLEAVED>
+__device__ __forceinline__ void rope_turn(RopeRaw<T, V>& x, RopeRaw<T, V>& y, const float (&cs)[V], const float (&sn)[V], int n) {
+  float p[V], q[V];
+  rope_unpack<T, V>(x, p);
+  rope_unpack<T, V>(y, q);
+  if constexpr (INTERLEAVED && V > 1) {
+#pragma unroll
+    for (int j = 0; j < V; j += 2) {
+      const int f = j / 2, s = V / 2 + j / 2;
+      const float p0 = p[j], q0 = q[j];
+      if (f < n) { p[j] = p0 * cs[f] - p[j + 1] * sn[f]; p[j + 1] = p[j + 1] * cs[f] + p0 * sn[f]; }
+      if (s < n) { q[j] = q0 * cs[s] - q[j + 1] * sn[s]; q[j + 1] = q[j + 1] * cs[s] + q0 * sn[s]; }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float p0 = p[j];
+      p[j] = p0 * cs[j] - q[j] * sn[j];
+      q[j] = q[j] * cs[j] + p0 * sn[j];
+    }
+  }
+  RopeRaw<T, V> rx = rope_pack<T, V>(p), ry = rope_pack<T, V>(q);
+  if constexpr (INTERLEAVED && V > 1 && sizeof(T) == 2) {       // what stays, stays bit by bit: a NaN's bits do not survive the conversion
+    const uint32_t *x0 = reinterpret_cast<const uint32_t*>(&x), *y0 = reinterpret_cast<const uint32_t*>(&y);
+#pragma unroll
+    for (int f = 0; f < V / 2; ++f) {
+      if (f >= n) reinterpret_cast<uint32_t*>(&rx)[f] = x0[f];
+      if (V / 2 + f >= n) reinterpret_cast<uint32_t*>(&ry)[f] = y0[f];
+    }
+  }
+  x = rx;
+  y = ry;
 }
 
 template <typename T, int V, bool INTERLEAVED>
-__global__ void __launch_bounds__(RT) rope_heads_kernel(const RopeArgs a) {
+__global__ void __launch_bounds__(RT, 3) rope_heads_kernel(const RopeArgs a) {
+  constexpr int R_HEADS = sizeof(T) * V >= 8 ? 4 : 8;        // heads in flight
   const unsigned int total = (unsigned int)(a.rows * a.units * a.groups);
   for (unsigned int i = blockIdx.x * RT + threadIdx.x; i < total; i += gridDim.x * RT) {
     const unsigned int g = i / a.units, unit = i - g * a.units;
@@ -80,25 +129,24 @@ __global__ void __launch_bounds__(RT) rope_heads_kernel(const RopeArgs a) {
     const long long row = a.row0 + r;
     const long long outer = row / a.inner, inner = row - outer * a.inner;
     const bool rotates = (int)unit < a.rot_units;
-    // element offsets of the two vectors of this unit inside a head; `two`: the second one is there
-    const int c = (int)unit * V;
+    // element offsets of the two vectors of this unit inside a head; `two`: the second one is there; n: pairs that are turned
+    const int c = (int)unit * V, n = min(V, a.half - c);
     int e0, e1;
-    bool two = true;
     if (rotates) {
       e0 = INTERLEAVED ? 2 * c : c;
       e1 = INTERLEAVED ? 2 * c + V : c + a.half;
     } else {
-      e0 = 2 * a.half + 2 * V * ((int)unit - a.rot_units);
+      e0 = (INTERLEAVED ? 2 * V * a.rot_units : 2 * a.half) + 2 * V * ((int)unit - a.rot_units);
       e1 = e0 + V;
-      two = e1 < a.d;
-      if (!two) e1 = e0;
     }
+    const bool two = e1 < a.d;
+    if (!two) e1 = e0;
     float cs[V], sn[V];
     if (rotates) {
       const double p = a.pos64 ? (double)reinterpret_cast<const long long*>(a.pos)[row] : (double)reinterpret_cast<const int*>(a.pos)[row];
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        const double turns = p * a.freq[c + j] * 0.15915494309189533577;      // 1 / (2 pi)
+        const double turns = p * a.freq[min(c + j, a.half - 1)] * 0.15915494309189533577;      // 1 / (2 pi)
         float s, k;
         sincospif((float)(2.0 * (turns - rint(turns))), &s, &k);
         cs[j] = k * a.scale;
@@ -109,36 +157,29 @@ __global__ void __launch_bounds__(RT) rope_heads_kernel(const RopeArgs a) {
       for (int j = 0; j < V; ++j) { cs[j] = 1.f; sn[j] = 0.f; }
     }
     const int all = a.heads[0] + a.heads[1];
-    for (int h = (int)group; h < all; h += a.groups) {
-      const int w = h >= a.heads[0];
-      const int hh = w ? h - a.heads[0] : h;
-      const RopeTensor& t = a.t[w];
-      const T* src = reinterpret_cast<const T*>(t.in) + outer * t.is0 + inner * t.is1 + hh * t.ish;
-      T* dst = reinterpret_cast<T*>(t.out) + outer * t.os0 + inner * t.os1 + hh * t.osh;
-      const RopeVec<T, V> x = rope_load<T, V>(src + e0), y = rope_load<T, V>(src + e1);
-      RopeVec<T, V> ox = x, oy = y;
-      if (rotates) {
-        if (INTERLEAVED && V > 1) {
+    for (int first = (int)group; first < all; first += R_HEADS * a.groups) {
+      RopeRaw<T, V> x[R_HEADS], y[R_HEADS];
 #pragma unroll
-          for (int j = 0; j < V; j += 2) {        // x holds the first V/2 pairs, y the others
-            const float p0 = rope_f(x.e[j]), p1 = rope_f(x.e[(j + 1) % V]), q0 = rope_f(y.e[j]), q1 = rope_f(y.e[(j + 1) % V]);
-            const int f = j / 2, s = V / 2 + j / 2;
-            ox.e[j] = rope_t<T>(p0 * cs[f] - p1 * sn[f]);
-            ox.e[(j + 1) % V] = rope_t<T>(p1 * cs[f] + p0 * sn[f]);
-            oy.e[j] = rope_t<T>(q0 * cs[s] - q1 * sn[s]);
-            oy.e[(j + 1) % V] = rope_t<T>(q1 * cs[s] + q0 * sn[s]);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < V; ++j) {
-            const float p = rope_f(x.e[j]), q = rope_f(y.e[j]);
-            ox.e[j] = rope_t<T>(p * cs[j] - q * sn[j]);
-            oy.e[j] = rope_t<T>(q * cs[j] + p * sn[j]);
-          }
-        }
+      for (int u = 0; u < R_HEADS; ++u) {
+        const int h = first + u * a.groups;
+        if (h >= all) continue;
+        const int w = h >= a.heads[0];
+        const RopeTensor& t = a.t[w];
+        const T* src = reinterpret_cast<const T*>(t.in) + outer * t.is0 + inner * t.is1 + (w ? h - a.heads[0] : h) * t.ish;
+        x[u] = *reinterpret_cast<const RopeRaw<T, V>*>(src + e0);
+        y[u] = *reinterpret_cast<const RopeRaw<T, V>*>(src + e1);
       }
-      rope_store<T, V>(dst + e0, ox);
-      if (two) rope_store<T, V>(dst + e1, oy);
+#pragma unroll
+      for (int u = 0; u < R_HEADS; ++u) {
+        const int h = first + u * a.groups;
+        if (h >= all) continue;
+        const int w = h >= a.heads[0];
+        const RopeTensor& t = a.t[w];
+        T* dst = reinterpret_cast<T*>(t.out) + outer * t.os0 + inner * t.os1 + (w ? h - a.heads[0] : h) * t.osh;
+        if (rotates) rope_turn<T, V, INTERLEAVED>(x[u], y[u], cs, sn, n);
+        *reinterpret_cast<RopeRaw<T, V>*>(dst + e0) = x[u];
+        if (two) *reinterpret_cast<RopeRaw<T, V>*>(dst + e1) = y[u];
+      }
     }
   }
 }
@@ -176,9 +217,10 @@ int dh_rope_heads(const void* call) {
   if (rows == 0 || heads_q + heads_k == 0) return 0;
   const int size = c.f32 ? 4 : 2;
   const bool in_place = (heads_q == 0 || ptrs[0] == ptrs[1]) && (heads_k == 0 || ptrs[2] == ptrs[3]);
-  // the widest vector that divides half the rotated part, the rest, every address and every stride
-  uint64_t odd = (uint64_t)(rotated / 2) * size;
-  if (!in_place) odd |= (uint64_t)(d - rotated) * size;
+  const int interleaved = (int)c.interleaved;
+  // the widest vector that divides every address and stride, and a head (interleaved) or half the rotated part and the rest (in halves)
+  uint64_t odd = (uint64_t)(interleaved ? d : rotated / 2) * size;
+  if (!interleaved && !in_place) odd |= (uint64_t)(d - rotated) * size;
   for (int i = 0; i < 4; ++i) {
     if ((i < 2 ? heads_q : heads_k) == 0) continue;
     odd |= (uint64_t)ptrs[i];
@@ -205,11 +247,11 @@ int dh_rope_heads(const void* call) {
   a.inner = (int)inner;
   a.half = rotated / 2;
   a.d = d;
-  a.rot_units = a.half / V;
-  a.units = a.rot_units + (in_place ? 0 : (d - rotated + 2 * V - 1) / (2 * V));
+  a.rot_units = (a.half + V - 1) / V;
+  const int rest = interleaved ? d - 2 * V * a.rot_units : d - rotated;
+  a.units = a.rot_units + (in_place || rest <= 0 ? 0 : (rest + 2 * V - 1) / (2 * V));
   const int sms = dh_sm_count();
   const int budget = (c.budget <= 0 || c.budget > sms) ? sms : (int)c.budget;
-  const int interleaved = (int)c.interleaved;
   const cudaStream_t s = (cudaStream_t)c.stream;
   // threads that share the heads of a row: enough of them to fill half of the GPU's threads, where there are that few rows
   a.groups = 1;
