@@ -61,6 +61,13 @@ def _add_megatron_args(parser):
     g.add_argument("--swiglu", action="store_true")
     g.add_argument("--position-embedding-type", default="rope", choices=["rope", "learned_absolute"])
     g.add_argument("--rotary-base", type=float, default=500000.0)
+    g.add_argument("--rotary-percent", type=float, default=1.0, help="first part of every head that is rotated")
+    g.add_argument("--rotary-interleaved", action="store_true", help="pairs (2i, 2i + 1) instead of (i, i + half)")
+    g.add_argument("--rotary-seq-len-interpolation-factor", type=float, default=None, help="positions interpolated by this factor")
+    g.add_argument("--use-rope-scaling", action="store_true", help="frequencies stretched to longer contexts")
+    g.add_argument("--rope-scaling-factor", type=float, default=8.0)
+    g.add_argument("--rope-scaling-type", default="llama3", choices=["linear", "ntk", "llama3", "yarn"])
+    g.add_argument("--rope-original-max-position", type=int, default=8192, help="positions of the first training")
     g.add_argument("--hidden-dropout", type=float, default=0.0)
     g.add_argument("--attention-dropout", type=float, default=0.0)
     g.add_argument("--untie-embeddings-and-output-weights", action="store_true")
@@ -93,6 +100,11 @@ def _add_megatron_args(parser):
     t.add_argument("--hysteresis", type=int, default=2)
     t.add_argument("--min-loss-scale", type=float, default=1.0)
     t.add_argument("--label-smoothing-factor", type=float, default=0.0)
+    t.add_argument("--distill-alpha", type=float, default=0.0,
+                   help="share of the distillation loss against a teacher's top logits (0: cross entropy alone)")
+    t.add_argument("--distill-temperature", type=float, default=1.0)
+    t.add_argument("--distill-top-k", type=int, default=16, help="the teacher's entries of a token")
+    t.add_argument("--distill-data", default=None, help="prefix of the teacher's .ids (int32) and .logits (float16) files beside --data-path")
     t.add_argument("--deterministic-mode", action="store_true", help="fixed-order reductions: two runs give bitwise equal results")
     t.add_argument("--use-distributed-optimizer", action="store_true")
     t.add_argument("--seed", type=int, default=1234)
@@ -148,12 +160,15 @@ def configs_from_args(args, world_size: int):
     """(ModelConfig, ParallelConfig, TrainConfig) from a Megatron-style namespace."""
     nq = args.num_attention_heads
     groups = args.num_query_groups if (args.group_query_attention and args.num_query_groups) else nq
+    scaling = ("linear", args.rotary_seq_len_interpolation_factor) if args.rotary_seq_len_interpolation_factor else \
+        (args.rope_scaling_type, args.rope_scaling_factor) if args.use_rope_scaling else ("none", 1.0)
     cfg = ModelConfig(
         name="megatron-args", num_layers=args.num_layers, hidden_size=args.hidden_size, ffn_hidden_size=args.ffn_hidden_size,
         num_attention_heads=nq, num_query_groups=groups, head_dim=args.kv_channels, vocab_size=args.vocab_size,
         seq_length=args.seq_length, norm="rmsnorm" if args.normalization == "RMSNorm" else "layernorm",
         activation="swiglu" if args.swiglu else "gelu", position="rope" if args.position_embedding_type == "rope" else "learned",
-        rope_theta=args.rotary_base, norm_eps=args.norm_epsilon, hidden_dropout=args.hidden_dropout,
+        rope_theta=args.rotary_base, rotary_percent=args.rotary_percent, rotary_interleaved=args.rotary_interleaved,
+        rope_scaling=scaling[0], rope_scaling_factor=scaling[1], rope_original_max_position=args.rope_original_max_position, norm_eps=args.norm_epsilon, hidden_dropout=args.hidden_dropout,
         tie_embeddings=not args.untie_embeddings_and_output_weights, init_std=args.init_method_std,
         num_experts=args.num_experts or 0, moe_top_k=args.moe_router_topk, moe_aux_loss_coeff=args.moe_aux_loss_coeff)
     tp, pp, cp = args.tensor_model_parallel_size, args.pipeline_model_parallel_size, args.context_parallel_size
@@ -171,7 +186,8 @@ def configs_from_args(args, world_size: int):
         loss_scale=args.loss_scale if args.loss_scale is not None else 1.0,
         dynamic_loss_scale=bool(args.fp16) and args.loss_scale is None, initial_loss_scale=args.initial_loss_scale,
         loss_scale_window=args.loss_scale_window, hysteresis=args.hysteresis, min_loss_scale=args.min_loss_scale,
-        label_smoothing=args.label_smoothing_factor, deterministic=args.deterministic_mode)
+        label_smoothing=args.label_smoothing_factor, distill_alpha=args.distill_alpha, distill_temperature=args.distill_temperature,
+        distill_top_k=args.distill_top_k, deterministic=args.deterministic_mode)
     return cfg, pcfg, train
 
 

@@ -26,6 +26,11 @@ class ModelConfig:
     activation: str = "swiglu"           # swiglu | gelu
     position: str = "rope"               # rope | learned
     rope_theta: float = 10000.0
+    rotary_percent: float = 1.0          # first part of every head that is rotated
+    rotary_interleaved: bool = False     # pairs (2i, 2i + 1) instead of (i, i + half)
+    rope_scaling: str = "none"           # none | linear | ntk | llama3 | yarn: frequencies stretched to longer contexts
+    rope_scaling_factor: float = 1.0
+    rope_original_max_position: int = 8192
     norm_eps: float = 1e-5
     hidden_dropout: float = 0.0
     tie_embeddings: bool = True          # the reference ties the LM head to the embedding (core/dshb.py:256-262)
@@ -38,6 +43,17 @@ class ModelConfig:
     def __post_init__(self):
         if self.head_dim is None:
             self.head_dim = self.hidden_size // self.num_attention_heads
+        if self.position == "rope" and (self.rotary_dim <= 0 or self.rotary_dim % 2 or self.rotary_dim > self.head_dim):
+            raise ValueError(f"rotary_percent {self.rotary_percent} of a head of {self.head_dim} is no even number of elements")
+
+    @property
+    def rotary_dim(self) -> int:
+        return int(self.head_dim * self.rotary_percent)
+
+    @property
+    def plain_rope(self) -> bool:
+        """Whole heads in halves at the frequencies of ``rope_theta``: what a table of all positions holds."""
+        return self.rotary_dim == self.head_dim and not self.rotary_interleaved and self.rope_scaling == "none"
 
     @property
     def is_moe(self) -> bool:
@@ -139,11 +155,21 @@ class TrainConfig:
     hysteresis: int = 2
     min_loss_scale: float = 1.0
     label_smoothing: float = 0.0         # Megatron's --label-smoothing-factor
+    # distillation from a teacher's top logits: loss = (1 - alpha) cross entropy + alpha temperature^2 KL(teacher || student)
+    distill_alpha: float = 0.0
+    distill_temperature: float = 1.0
+    distill_top_k: int = 16              # entries a token of synthetic teachers
     # the two switches of the benchmark's composition arm: the reference's built-in 17-block schedule
     # (dhellam/core/dstb.py:1043-1059) and its device-wide synchronisation after every block (:1266)
     reference_schedule: bool = False
     sync_per_block: bool = False
     deterministic: bool = False          # Megatron's --deterministic-mode: fixed-order reductions, bitwise repeatable runs
+
+    def __post_init__(self):
+        if not 0.0 <= self.distill_alpha <= 1.0 or not 0.0 < self.distill_temperature < float("inf"):
+            raise ValueError("distillation needs an alpha between 0 and 1 and a positive temperature")
+        if self.distill_alpha and self.label_smoothing:
+            raise ValueError("label smoothing and distillation from a teacher exclude each other")
 
     def num_microbatches(self, dp: int) -> int:
         assert self.global_batch_size % (self.micro_batch_size * dp) == 0, "global batch must divide by micro-batch x dp"

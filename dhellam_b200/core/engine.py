@@ -26,7 +26,7 @@ import torch
 from ..config import ModelConfig, TrainConfig
 from ..models import head as H
 from ..models.transformer import build_layer_program
-from ..ops.rope import rope_table
+from ..ops.rope import RopeScaling, rope_frequencies, rope_table
 from ..parallel import pp as PP
 from ..sched.executor import Executor, StreamSet
 from ..sched.ir import LayerRun
@@ -44,6 +44,9 @@ class MicroBatch:
     batch: int
     seed: int = 0
     positions_local: Optional[torch.Tensor] = None   # [T/t] positions of this rank's sequence-parallel rows
+    token_mask: Optional[torch.Tensor] = None        # [T] bool: rows that count in the router's balance (None: all)
+    teacher_ids: Optional[torch.Tensor] = None       # [T, K] integer: the teacher's best entries of each row (distillation)
+    teacher_logits: Optional[torch.Tensor] = None    # [T, K]
 
 
 class Env:
@@ -60,11 +63,16 @@ class Env:
         self.cur_stream = None
         self.exposed = None           # ExposedTimer of the engine's executor (set by the engine)
         self.softmax_scale = 1.0 / math.sqrt(cfg.head_dim)
-        self.rope_cos = self.rope_sin = None
-        if cfg.position == "rope":
+        self.rope_cos = self.rope_sin = self.rope_freq = None
+        self.rope_scale = 1.0
+        if cfg.position == "rope" and not cfg.plain_rope:
+            scaling = None if cfg.rope_scaling == "none" else RopeScaling(cfg.rope_scaling, cfg.rope_scaling_factor, cfg.rope_original_max_position)
+            self.rope_freq, self.rope_scale = rope_frequencies(cfg.rotary_dim, cfg.rope_theta, scaling, self.device)
+        elif cfg.position == "rope":
             c, s = rope_table(cfg.seq_length, cfg.head_dim, cfg.rope_theta)
             self.rope_cos, self.rope_sin = c.to(self.device), s.to(self.device)
         self.moe_aux = []             # auxiliary (load-balance) losses of the current step
+        self.moe_counts = []          # choices per expert [E] int32 of every router call of the current step
 
 
 def hand_over(obj, stream):
@@ -316,6 +324,7 @@ class DoubleStrandEngine:
         N = len(mbs)
         self.losses = []
         self.env.moe_aux = []
+        self.env.moe_counts = []
         self.grad_scale = self.loss_scale / N
         self.env.grad_scale = self.grad_scale
         st = self.streams

@@ -334,10 +334,6 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
         }
       }
     };
-    const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
-    const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
-    const bool lin = lloc >= 0 && lloc < a.Vl;
-    const float zl = lin ? d_load(z + lloc) : 0.f;
     int stage = 0;
     for (int k = 0; k < full; ++k, stage = STAGE - stage) {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -346,6 +342,10 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     }
     asm volatile("cp.async.wait_group 1;" ::: "memory");
     if (left > 0) batch(stage, left);
+    const float z0 = id0 - a.v0 >= 0 && id0 - a.v0 < a.Vl ? d_load(z + (id0 - a.v0)) : 0.f;
+    const int lloc = lab >= 0 && lab < a.V ? lab - a.v0 : -1;
+    const bool lin = lloc >= 0 && lloc < a.Vl;
+    const float zl = lin ? d_load(z + lloc) : 0.f;
     float s1, st;
     acc.finish(c1, ct, s1, st);
     // elements one by one: before the first and behind the last vector

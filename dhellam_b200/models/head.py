@@ -111,14 +111,22 @@ def embed_bwd(env, hp: HeadParams, mb, dx):
 
 
 def loss_fwd(env, hp: HeadParams, mb, x):
-    """final norm -> gather -> logits -> vocab-parallel CE -> masked mean.
-    Returns ``(loss scalar tensor, saved)``."""
+    """final norm -> gather -> logits -> vocab-parallel CE -> masked mean.  With a teacher's top logits in the micro-batch the loss is
+    ``(1 - alpha)`` of that and ``alpha`` of the distillation loss.  Returns ``(loss scalar tensor, saved)``."""
     x = _use(env, x)
     y, stat = _norm_fwd(env, x, hp.final_ln_weight, hp.get("final_ln_bias"), 0)
     y_full = tp_gather_rows(env, y, "head")        # a staging-buffer view: valid until the second next head gather
     logits = G.gemm_nt(y_full, hp.lm_weight)
     v0, _ = vocab_range(env)
-    loss_tok, lse = L.vocab_parallel_ce_fwd(logits, mb.labels, v0, env.ps.tp_group, label_smoothing=env.train.label_smoothing)
+    alpha = env.train.distill_alpha
+    if alpha:
+        if mb.teacher_ids is None:
+            raise ValueError("distillation (distill_alpha > 0) needs a teacher's top logits in every micro-batch")
+        ce, kd, lse = L.vocab_parallel_distill_fwd(logits, mb.labels, mb.teacher_ids, mb.teacher_logits, env.train.distill_temperature, v0,
+                                                   env.ps.tp_group)
+        loss_tok = (1.0 - alpha) * ce + alpha * kd
+    else:
+        loss_tok, lse = L.vocab_parallel_ce_fwd(logits, mb.labels, v0, env.ps.tp_group, label_smoothing=env.train.label_smoothing)
     mask = mb.loss_mask.reshape(-1).float()
     sums = torch.stack([(loss_tok * mask).sum(), mask.sum()])
     if env.ps.cp > 1:
@@ -133,8 +141,13 @@ def loss_bwd(env, hp: HeadParams, mb, saved, grad_scale: float):
     v0, _ = vocab_range(env)
     g_tok = L.mask_scale_loss_bwd(mb.loss_mask, saved["count"], grad_scale)
     logits = _use(env, saved.pop("logits"))
-    dlogits = L.vocab_parallel_ce_bwd_(logits, mb.labels, _use(env, saved.pop("lse")), g_tok, v0,
-                                       label_smoothing=env.train.label_smoothing, vocab=env.cfg.vocab_size)
+    alpha, stat = env.train.distill_alpha, _use(env, saved.pop("lse"))
+    if alpha:
+        dlogits = L.vocab_parallel_distill_bwd_(logits, mb.labels, mb.teacher_ids, mb.teacher_logits, stat, (1.0 - alpha) * g_tok,
+                                                alpha * g_tok, env.train.distill_temperature, v0)
+    else:
+        dlogits = L.vocab_parallel_ce_bwd_(logits, mb.labels, stat, g_tok, v0, label_smoothing=env.train.label_smoothing,
+                                           vocab=env.cfg.vocab_size)
     if dlogits.dtype != hp.lm_weight.dtype:
         dlogits = dlogits.to(hp.lm_weight.dtype)
     y_full = _use(env, saved.pop("y_full"))

@@ -43,7 +43,9 @@ def f_router(run):
     probs, topi, gates = M.router_topk_fwd(x, p.router_weight, env.cfg.moe_top_k)
     run.acts["moe_x"], run.acts["moe_probs"], run.acts["moe_topi"], run.acts["moe_gates"] = x, probs, topi, gates
     if env.training and env.cfg.moe_aux_loss_coeff > 0:
-        env.moe_aux.append(M.aux_loss(probs, topi, env.cfg.num_experts))
+        loss, counts, run.acts["moe_balance"] = M.balance_loss_fwd(probs, topi, getattr(run.mb, "token_mask", None))
+        env.moe_aux.append(loss)
+        env.moe_counts.append(counts)
     run.v["moe_x"] = x
 
 
@@ -263,7 +265,8 @@ def b_router_bwd(run):
     probs, topi, gates = run.acts.pop("moe_probs"), run.acts.pop("moe_topi"), run.acts.pop("moe_gates")
     run.acts.pop("moe_plan")
     aux_scale = env.cfg.moe_aux_loss_coeff * getattr(env, "grad_scale", 1.0) if env.training else 0.0
-    d_logits = M.router_topk_bwd(run.v.pop("d_gates"), probs, topi, gates, env.cfg.num_experts, aux_scale)
+    d_logits = M.router_topk_bwd(run.v.pop("d_gates"), probs, topi, gates, env.cfg.num_experts, aux_scale,
+                                 balance=run.acts.pop("moe_balance", None))
     dl = d_logits.to(x.dtype)
     d_x = run.v.pop("d_moe_x")
     E = dl.shape[1]

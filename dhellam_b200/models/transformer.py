@@ -173,6 +173,12 @@ def _apply_rope(run, qkv, inverse=False):
     if env.cfg.position != "rope":
         return
     nq, nkv, d = _heads(env)
+    if env.rope_freq is not None:
+        heads = qkv.view(qkv.shape[0], nq + 2 * nkv, d)
+        q, k = heads[:, :nq], heads[:, nq:nq + nkv]
+        turn = R.rope_bwd if inverse else R.rope_fwd
+        turn(q, k, run.mb.positions, env.rope_freq, interleaved=env.cfg.rotary_interleaved, scale=env.rope_scale, out=(q, k))
+        return
     R.rope_apply_(qkv, run.mb.positions, env.rope_cos, env.rope_sin, nq, nkv, d, inverse=inverse)
 
 

@@ -142,6 +142,11 @@ class Trainer:
             return loss
         return None
 
+    def expert_load(self):
+        """Choices per expert ``[E]`` of the last step on this rank, over its router calls (``None`` without a balance loss)."""
+        counts = self.env.moe_counts
+        return torch.stack(counts).sum(0) if counts else None
+
     def close(self):
         """Drops every reference this trainer (and the module-level blackboard) holds to the model,
         the optimizer state and the symmetric buffers, so that their device memory can be freed

@@ -40,7 +40,7 @@ def main(argv=None):
     from dhellam_b200.adaptor import initialize_dhellam_megatron
     from dhellam_b200.ckpt import load_checkpoint, save_checkpoint
     from dhellam_b200.common import print_rank0
-    from dhellam_b200.data import TokenFileDataset, file_step_batches, synthetic_step_batches
+    from dhellam_b200.data import TeacherTopFile, TokenFileDataset
     from dhellam_b200.runtime.metrics import MetricsLogger
     from dhellam_b200.trainer import Trainer
 
@@ -67,7 +67,8 @@ def main(argv=None):
     if args.data_path and not args.mock_data:
         # a flat token file (the payload of a Megatron .bin file); "<path>:<dtype>" selects the id type
         path, _, dt = args.data_path[-1].partition(":")
-        dataset = TokenFileDataset(path, cfg.seq_length, dt or "int32", seed=train.seed)
+        teacher = TeacherTopFile(args.distill_data, train.distill_top_k) if args.distill_data else None
+        dataset = TokenFileDataset(path, cfg.seq_length, dt or "int32", seed=train.seed, teacher=teacher)
         print_rank0(f"data: {path} ({len(dataset)} samples of {cfg.seq_length + 1} tokens)")
     tr.engine.time_pp = pcfg.pp > 1 and args.timing_log_level >= 2
     # Failure detection between steps: every rank beats on the rendezvous store and announces the
@@ -134,7 +135,10 @@ def _loop(args, tr, train, cfg, pcfg, dataset, device, cuda, start, ml, hb, gate
             dist.all_reduce(t, op=dist.ReduceOp.MAX)
             ms = float(t)
         lv = float(loss) if loss is not None else None
-        extra = {"pp_bubble_ms": tr.engine.pp_bubble_ms()} if tr.engine.time_pp else None
+        extra = {"pp_bubble_ms": tr.engine.pp_bubble_ms()} if tr.engine.time_pp else {}
+        load = tr.expert_load()
+        if load is not None:               # the busiest expert's share against an even one
+            extra["expert_load_max_over_mean"] = float(load.max() / load.float().mean().clamp_min(1e-9))
         rec = ml.log(it + 1, ms, lv, float(tr.last_grad_norm) if tr.last_grad_norm is not None else None, extra)
         if (it + 1) % train.log_interval == 0:
             print_rank0(f" iteration {it + 1:6d}/{train.train_iters} | elapsed time per iteration (ms): {ms:.1f} | lm loss: "
