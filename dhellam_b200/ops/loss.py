@@ -16,6 +16,7 @@ depend on the tensor-parallel size.
 """
 from __future__ import annotations
 
+import math
 import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 
@@ -120,6 +121,11 @@ MAX_TEACHER_ENTRIES = 1024
 
 
 def _distill_operands(what, logits, labels, top_ids, top_logits, temperature):
+    shape, ids, id_type = logits.shape, top_ids.shape, top_ids.dtype
+    if len(shape) == 2 and len(ids) == 2 and ids[0] == shape[0] and top_logits.shape == ids and (id_type is torch.int32 or id_type is torch.int64) \
+            and top_logits.dtype in _TEACHER_TYPES and ids[1] <= MAX_TEACHER_ENTRIES and 0.0 < temperature < math.inf \
+            and (labels is None or (labels.dtype is torch.int32 and labels.shape == shape[:1])):
+        return
     if logits.dim() != 2 or top_ids.dim() != 2 or top_ids.shape[0] != logits.shape[0] or top_logits.shape != top_ids.shape:
         raise ValueError(f"{what}: logits [T, V], the teacher's ids and logits [T, K], got {tuple(logits.shape)}, {tuple(top_ids.shape)}, "
                          f"{tuple(top_logits.shape)}")
@@ -139,21 +145,24 @@ def _distill_native(what, logits, labels, top_ids, top_logits, *others):
     if logits.stride(1) != 1 and logits.shape[1] > 1:
         raise ValueError(f"{what}: the logits of a row lie side by side")
     K.require_current_device(what, logits, labels, top_ids, top_logits, *others)
-    return (labels if labels is None or labels.is_contiguous() else labels.contiguous(),
-            top_ids if top_ids.stride(1) == 1 else top_ids.contiguous(),
-            top_logits if top_logits.stride(1) == 1 else top_logits.contiguous())
+    if labels is not None and not labels.is_contiguous():
+        labels = labels.contiguous()
+    return labels, top_ids if top_ids.stride(1) == 1 else top_ids.contiguous(), top_logits if top_logits.stride(1) == 1 else top_logits.contiguous()
 
 
 # The operands of both kernels as one block of 8-byte fields (DistillCall in csrc/distill.cu): ctypes converts argument by argument,
 # which takes 2 us where a small call has 12 in all.
 _DISTILL_CALL = struct.Struct("=17qd")
+_DISTILL_FWD = [c_void_p] * 5
+_DISTILL_BWD = [c_void_p] * 5 + [c_int64]
 
 
 def _distill_call(logits, labels, ids, top, vocab_start, vocab, temperature, sm_budget):
     T, Vl = logits.shape
-    return _DISTILL_CALL.pack(logits.data_ptr(), logits.stride(0), logits.dtype == torch.float32, K.ptr(labels), ids.data_ptr(), ids.stride(0),
-                              ids.dtype == torch.int64, top.data_ptr(), top.stride(0), _TEACHER_TYPES[top.dtype], T, Vl, ids.shape[1],
-                              vocab_start, vocab, sm_budget, K.current_raw_stream(), temperature)
+    return _DISTILL_CALL.pack(logits.data_ptr(), logits.stride()[0], logits.dtype is torch.float32, labels.data_ptr() if labels is not None else 0,
+                              ids.data_ptr(), ids.stride()[0], ids.dtype is torch.int64, top.data_ptr(), top.stride()[0],
+                              _TEACHER_TYPES[top.dtype], T, Vl, ids.shape[1], vocab_start, vocab, sm_budget,
+                              torch._C._cuda_getCurrentRawStream(logits.get_device()), temperature)
 
 
 def _teacher_ref(top_ids, top_logits, vocab, temperature):
@@ -230,7 +239,7 @@ def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature:
     if native:
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits)
         call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature, sm_budget)
-        fn = K.proto("dh_distill_fwd", [c_void_p] * 5)
+        fn = K.proto("dh_distill_fwd", _DISTILL_FWD)
         kd = logits.new_empty(T, dtype=torch.float32)
         ce = torch.empty_like(kd) if labels is not None else None
         saved = logits.new_empty((T, 4), dtype=torch.float32)
@@ -264,20 +273,24 @@ def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce
     _distill_operands(what, logits, labels, top_ids, top_logits, temperature)
     T, Vl = logits.shape
     out = logits if out is None else out
-    if out.shape != logits.shape or out.dtype != logits.dtype or (out.stride(0) < Vl and T > 1) or (out.stride(1) != 1 and Vl > 1):
-        raise ValueError(f"{what}: an output of the logits' shape and type with room for every row, got {out.dtype} {tuple(out.shape)}")
-    if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
-            and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
-        raise ValueError(f"{what}: the output is the logits themselves or shares no memory with them")
+    if out is not logits:
+        row, column = out.stride()
+        if out.shape != logits.shape or out.dtype != logits.dtype or (row < Vl and T > 1) or (column != 1 and Vl > 1):
+            raise ValueError(f"{what}: an output of the logits' shape and type with room for every row, got {out.dtype} {tuple(out.shape)}")
+        if out.untyped_storage().data_ptr() == logits.untyped_storage().data_ptr() \
+                and (out.data_ptr() != logits.data_ptr() or out.stride() != logits.stride()):
+            raise ValueError(f"{what}: the output is the logits themselves or shares no memory with them")
+    elif T > 1 and logits.stride(0) < Vl:
+        raise ValueError(f"{what}: logits that are overwritten have room for every row")
     if (g_ce is None) != (labels is None):
         raise ValueError(f"{what}: labels and the gradient of their loss go together")
-    for t, shape in ((g_ce, (T,)), (g_kd, (T,)), (saved, (T, 4))):
-        if t is not None and (t.shape != shape or t.dtype != torch.float32 or not t.is_contiguous()):
+    for t in (g_kd, g_ce, saved):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != ((T, 4) if t is saved else (T,)) or not t.is_contiguous()):
             raise ValueError(f"{what}: contiguous fp32 gradients [T] and saved statistics [T, 4], got {t.dtype} {tuple(t.shape)}")
     if K.use_native(logits):
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out)
         call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature, sm_budget)
-        fn = K.proto("dh_distill_bwd", [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64])
+        fn = K.proto("dh_distill_bwd", _DISTILL_BWD)
         K.check(fn(call, saved.data_ptr(), K.ptr(g_ce), g_kd.data_ptr(), out.data_ptr(), out.stride(0)), what)
         return out
     rel = logits.float() - saved[:, :1]

@@ -49,12 +49,13 @@ class Balance(NamedTuple):
 
 
 def _router_operands(what, probs, topi, mask):
-    if probs.dim() != 2 or topi.dim() != 2 or topi.shape[0] != probs.shape[0] or probs.dtype != torch.float32 \
-            or topi.dtype not in (torch.int32, torch.int64) or not topi.shape[1]:
+    shape, ids, id_type = probs.shape, topi.shape, topi.dtype
+    if len(shape) != 2 or len(ids) != 2 or ids[0] != shape[0] or probs.dtype is not torch.float32 \
+            or (id_type is not torch.int32 and id_type is not torch.int64) or not ids[1]:
         raise ValueError(f"{what}: fp32 probabilities [T, E] and int32 or int64 choices [T, k], got {probs.dtype} {tuple(probs.shape)} "
                          f"and {topi.dtype} {tuple(topi.shape)}")
-    if mask is not None and (mask.shape != probs.shape[:1] or mask.dtype not in (torch.bool, torch.uint8)):
-        raise ValueError(f"{what}: a mask of {probs.shape[0]} bool or uint8 values, got {mask.dtype} {tuple(mask.shape)}")
+    if mask is not None and (mask.shape != shape[:1] or mask.dtype not in (torch.bool, torch.uint8)):
+        raise ValueError(f"{what}: a mask of {shape[0]} bool or uint8 values, got {mask.dtype} {tuple(mask.shape)}")
 
 
 def _on_kernel(probs, topi, *others):
@@ -67,12 +68,16 @@ def _on_kernel(probs, topi, *others):
 
 # The operands that both kernels share, as one block of 8-byte fields (BalCall in csrc/balance.cu): ctypes converts argument by argument.
 _ROUTER_CALL = struct.Struct("=11q")
+_SCRATCH = [c_void_p]
+_BALANCE_FWD = [c_void_p] * 5
+_ROUTER_BWD = [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p]
 
 
 def _router_call(probs, topi, mask, sm_budget):
     T, E = probs.shape
-    return _ROUTER_CALL.pack(probs.data_ptr(), probs.stride(0), topi.data_ptr(), topi.stride(0), topi.dtype == torch.int64, K.ptr(mask), T, E,
-                             topi.shape[1], sm_budget, K.current_raw_stream())
+    return _ROUTER_CALL.pack(probs.data_ptr(), probs.stride()[0], topi.data_ptr(), topi.stride()[0], topi.dtype is torch.int64,
+                             mask.data_ptr() if mask is not None else 0, T, E, topi.shape[1], sm_budget,
+                             torch._C._cuda_getCurrentRawStream(probs.get_device()))
 
 
 def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
@@ -92,13 +97,10 @@ def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
         if mask is not None and not mask.is_contiguous():
             mask = mask.contiguous()
         call = _router_call(probs, topi, mask, sm_budget)
-        out = probs.new_empty(2 * E + 1)
-        coef, loss, counts = out[:E], out[E], out[E + 1:].view(torch.int32)
-        words = K.proto("dh_balance_scratch", [c_void_p], c_int64)(call)
-        scratch = probs.new_empty(words) if words else None
-        base = out.data_ptr()
-        fn = K.proto("dh_balance_fwd", [c_void_p] * 5)
-        K.check(fn(call, K.ptr(scratch), base + 4 * E, base + 4 * (E + 1), base), "dh_balance_fwd")
+        loss, coef, counts = probs.new_empty(()), probs.new_empty(E), probs.new_empty(E, dtype=torch.int32)
+        words = K.proto("dh_balance_scratch", _SCRATCH, c_int64)(call)
+        scratch = probs.new_empty(words).data_ptr() if words else 0
+        K.check(K.proto("dh_balance_fwd", _BALANCE_FWD)(call, scratch, loss.data_ptr(), counts.data_ptr(), coef.data_ptr()), "dh_balance_fwd")
         return loss, counts, Balance(coef, mask)
     counted = torch.ones(T, dtype=torch.bool, device=probs.device) if mask is None else mask != 0
     n = counted.sum().clamp_min(1)
@@ -131,14 +133,22 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
         raise ValueError(f"router_topk_bwd: gates and their gradient as the choices {tuple(topi.shape)}, probabilities and balance of {E} "
                          f"experts")
     T, k = topi.shape
-    if _on_kernel(probs, topi, d_gates, gates, mask) and d_gates.dtype == gates.dtype == torch.float32:
-        if aux_scale and balance is None:
-            balance = balance_loss_fwd(probs, topi)[2]
-        topi, gates, d_gates = (t if t.stride(1) == 1 else t.contiguous() for t in (topi, gates, d_gates))
+    coef = balance.coef if balance is not None else None
+    if _on_kernel(probs, topi, d_gates, gates, mask, coef) and d_gates.dtype is gates.dtype is torch.float32 \
+            and (coef is None or coef.dtype is torch.float32):
+        if aux_scale and coef is None:
+            coef = balance_loss_fwd(probs, topi)[2].coef
+        if mask is not None and not mask.is_contiguous():
+            mask = mask.contiguous()
+        if coef is not None and not coef.is_contiguous():
+            coef = coef.contiguous()
+        (gs, gc), (ds, dc) = gates.stride(), d_gates.stride()
+        if k > 1 and not (gc == dc == 1 == topi.stride(1)):
+            topi, gates, d_gates = topi.contiguous(), gates.contiguous(), d_gates.contiguous()
+            gs = ds = k
         out = probs.new_empty((T, E))
-        fn = K.proto("dh_router_bwd", [c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_float, c_void_p])
-        K.check(fn(_router_call(probs, topi, mask, sm_budget), gates.data_ptr(), gates.stride(0), d_gates.data_ptr(), d_gates.stride(0),
-                   balance.coef.data_ptr() if aux_scale else 0, aux_scale, out.data_ptr()), "dh_router_bwd")
+        K.check(K.proto("dh_router_bwd", _ROUTER_BWD)(_router_call(probs, topi, mask, sm_budget), gates.data_ptr(), gs, d_gates.data_ptr(), ds,
+                                                      coef.data_ptr() if aux_scale else 0, aux_scale, out.data_ptr()), "dh_router_bwd")
         return out
     valid = (topi >= 0) & (topi < E)
     at = torch.where(valid, topi, torch.zeros_like(topi)).long()
@@ -148,9 +158,7 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
     d_probs = torch.zeros_like(probs)
     d_probs.scatter_add_(1, at, d_topv)
     if aux_scale:
-        if balance is None:
-            balance = balance_loss_fwd(probs, topi)[2]
-        d_aux = aux_scale * balance.coef[None, :]
+        d_aux = aux_scale * (balance_loss_fwd(probs, topi)[2].coef if coef is None else coef)[None, :]
         if mask is not None:
             d_aux = torch.where(mask[:, None] != 0, d_aux, torch.zeros_like(d_aux))
         d_probs = d_probs + d_aux

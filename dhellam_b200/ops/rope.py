@@ -126,6 +126,9 @@ def _turn_ref(x, positions, freq, interleaved, scale, transposed):
 # The operands of the kernel as one block of 8-byte fields (RopeCall in csrc/rope.cu): ctypes converts argument by argument, which takes
 # several microseconds where a small call has 15 in all.
 _ROPE_CALL = struct.Struct("=30qd")
+_ROPE_ARGS = [c_void_p]
+_TYPES = (torch.bfloat16, torch.float32)
+_POSITIONS = (torch.int32, torch.int64)
 
 
 def _fits(x, lead, d, dtype):
@@ -164,6 +167,29 @@ def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
         operands = (q, k, positions, freq) + (tuple(out) if out is not None else ())
         return K.run_on_stream(stream, operands, lambda: _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
                                                                None, what))
+    shape, dtype, pairs = q.shape, q.dtype, freq.numel()
+    if out is not None or k is None or len(shape) != 3 or not K.use_native(q):
+        return _turn_any(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget, what)
+    # packed rows on the GPU, outputs of their own: what `_turn_any` checks, asked once
+    T, heads, d = shape
+    kshape, (sq, hq, cq), (sk, hk, ck) = k.shape, q.stride(), k.stride() if k.dim() == 3 else (0, 0, 0)
+    device, pos_type = q.get_device(), positions.dtype
+    if not (dtype in _TYPES and k.dtype is dtype and cq == 1 and ck == 1 and kshape[0] == T and kshape[2] == d and positions.shape == (T,)
+            and pos_type in _POSITIONS and freq.dtype is torch.float64 and freq.dim() == 1 and 0 < 2 * pairs <= d
+            and device == k.get_device() == positions.get_device() == freq.get_device() == torch._C._cuda_getDevice()
+            and positions.is_contiguous() and freq.is_contiguous()):
+        return _turn_any(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget, what)
+    kv = kshape[1]
+    oq = torch.empty_like(q, memory_format=torch.contiguous_format)
+    ok = torch.empty_like(k, memory_format=torch.contiguous_format)
+    call = _ROPE_CALL.pack(q.data_ptr(), oq.data_ptr(), k.data_ptr(), ok.data_ptr(), sq, 0, hq, heads * d, 0, d, sk, 0, hk, kv * d, 0, d, heads,
+                           kv, positions.data_ptr(), pos_type is torch.int64, freq.data_ptr(), T, 1, d, 2 * pairs, bool(interleaved),
+                           dtype is torch.float32, transposed, sm_budget, torch._C._cuda_getCurrentRawStream(device), scale)
+    K.check(K.proto("dh_rope_heads", _ROPE_ARGS)(call), "dh_rope_heads")
+    return oq, ok
+
+
+def _turn_any(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget, what):
     _check(q, k, positions, freq, out, what)
     oq, ok = out if out is not None else (None, None)
     if not K.use_native(q):
@@ -171,7 +197,7 @@ def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
         rk = _turn_ref(k, positions, freq, interleaved, scale, transposed) if k is not None else None
         return (rq, rk) if out is None else (oq.copy_(rq), ok.copy_(rk) if k is not None else None)
     shape, dtype = q.shape, q.dtype
-    if dtype != torch.bfloat16 and dtype != torch.float32:
+    if dtype not in _TYPES:
         raise ValueError(f"{what}: the sm_100a kernel rotates bf16 and fp32, not {dtype}")
     K.require_current_device(what, q, k, positions, freq, oq, ok)
     if not positions.is_contiguous() or not freq.is_contiguous():
@@ -188,7 +214,7 @@ def _turn(q, k, positions, freq, interleaved, scale, out, transposed, sm_budget,
                            positions.data_ptr(), positions.dtype == torch.int64, freq.data_ptr(), positions.numel(),
                            1 if len(shape) == 3 else shape[1] or 1, shape[-1], 2 * freq.numel(), bool(interleaved), dtype == torch.float32,
                            transposed, sm_budget, K.current_raw_stream(), scale)
-    K.check(K.proto("dh_rope_heads", [c_void_p])(call), "dh_rope_heads")
+    K.check(K.proto("dh_rope_heads", _ROPE_ARGS)(call), "dh_rope_heads")
     return oq, ok
 
 

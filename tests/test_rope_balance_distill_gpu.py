@@ -217,6 +217,15 @@ def test_balance_choices_out_of_range_twice_and_without_balance():
     assert torch.equal(counted, M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=M.balance_loss_fwd(probs, ids)[2]))
 
 
+def test_router_gradient_with_a_strided_balance():
+    T, E, k = 64, 10, 2
+    probs, ids, gates, dg, mask = router_case(T, E, k, device=DEV)
+    bal = M.balance_loss_fwd(probs, ids, mask)[2]
+    want = M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=bal)
+    spread = M.Balance(torch.stack([bal.coef] * 2, 1)[:, 0], torch.stack([mask] * 3, 1)[:, 1])
+    assert torch.equal(want, M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=spread))
+
+
 def test_balance_on_another_stream_in_a_graph_and_with_a_budget():
     probs, ids, gates, dg, mask = router_case(3000, 40, 4, device=DEV)
 
