@@ -76,15 +76,18 @@ __global__ void __launch_bounds__(BF, 1024 / BF) balance_kernel(const BalArgs a,
   __syncthreads();
   const int64_t t0 = (int64_t)a.T * blockIdx.x / gridDim.x, t1 = (int64_t)a.T * (blockIdx.x + 1) / gridDim.x;
   const int n = (int)(t1 - t0);
+  int tokens = 0;
   for (int r = threadIdx.x; r < n; r += BF) {
     if (a.mask != nullptr && !a.mask[t0 + r]) continue;
-    atomicAdd(&cnt[a.E], 1);
+    ++tokens;
 #pragma unroll 4
     for (int j = 0; j < a.k; ++j) {
       const int e = bal_id(a, t0 + r, j);
       if (e >= 0) atomicAdd(&cnt[e], 1);
     }
   }
+  tokens = __reduce_add_sync(0xffffffffu, tokens);
+  if (lane == 0) atomicAdd(&cnt[a.E], tokens);
   // columns: the next power of two of E / W, at most BF
   const int groups = (a.E + W - 1) / W;
   int cols = 1;
@@ -266,6 +269,14 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
     const int64_t t = base + lane / L;
     const bool row = t < a.T;
     const float* p = a.probs + (row ? t : 0) * a.p_stride;
+    int id = -1;
+    float dg = 0.f, g = 0.f;
+    if (row && l < a.k) {
+      id = bal_id(a, t, l);
+      dg = b.d_gates[t * b.dg_stride + l];
+      g = b.gates[t * b.g_stride + l];
+    }
+    const bool counts = row && (a.mask == nullptr || a.mask[t] != 0);
     BalVec<W> v[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -274,15 +285,8 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
       for (int q = 0; q < W; ++q) v[i].v[q] = 0.f;
       if (row && e < a.E) v[i] = bal_load<W>(p + e);
     }
-    int id = -1;
-    float dot = 0.f, dg = 0.f, pj = 0.f;
-    if (row && l < a.k) {
-      id = bal_id(a, t, l);
-      dg = b.d_gates[t * b.dg_stride + l];
-      const float g = b.gates[t * b.g_stride + l];
-      if (id >= 0) { pj = p[id]; dot = dg * g; }
-    }
-    const bool counts = row && (a.mask == nullptr || a.mask[t] != 0);
+    float dot = 0.f, pj = 0.f;
+    if (id >= 0) { pj = p[id]; dot = dg * g; }
     float sel = pj;
     bal_group_sum<L>(dot, sel);
     float u = id >= 0 && sel != 0.f ? (dg - dot) / sel : 0.f;

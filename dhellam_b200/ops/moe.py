@@ -99,8 +99,8 @@ def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
         call = _router_call(probs, topi, mask, sm_budget)
         loss, coef, counts = probs.new_empty(()), probs.new_empty(E), probs.new_empty(E, dtype=torch.int32)
         words = K.proto("dh_balance_scratch", _SCRATCH, c_int64)(call)
-        scratch = probs.new_empty(words).data_ptr() if words else 0
-        K.check(K.proto("dh_balance_fwd", _BALANCE_FWD)(call, scratch, loss.data_ptr(), counts.data_ptr(), coef.data_ptr()), "dh_balance_fwd")
+        scratch = probs.new_empty(words) if words else None
+        K.check(K.proto("dh_balance_fwd", _BALANCE_FWD)(call, K.ptr(scratch), loss.data_ptr(), counts.data_ptr(), coef.data_ptr()), "dh_balance_fwd")
         return loss, counts, Balance(coef, mask)
     counted = torch.ones(T, dtype=torch.bool, device=probs.device) if mask is None else mask != 0
     n = counted.sum().clamp_min(1)
