@@ -132,6 +132,33 @@ def build(kernel, a):
         lg = bf(M, Nn, scale=3.0)
         lab = torch.randint(0, Nn, (M,), dtype=torch.int32, device="cuda")
         return (lambda: L.ce_local_stats(lg, lab, 0)), 0.0, 2.0 * M * Nn
+    if kernel in ("rope_fwd", "rope_bwd"):          # the packed projection of a sequence: queries and keys read, written to their own memory
+        from ..ops import rope as R
+        S, B, H, Hk, d = a.seq, a.batch, a.heads, a.kv_heads, 128
+        qkv = bf(S * B, H + 2 * Hk, d)
+        q, k = qkv[:, :H], qkv[:, H:H + Hk]
+        pos = torch.arange(S, dtype=torch.int32, device="cuda").repeat_interleave(B)
+        freq, scale = R.rope_frequencies(d, 500000.0, R.RopeScaling("llama3", 8.0), "cuda")
+        turn = R.rope_fwd if kernel == "rope_fwd" else R.rope_bwd
+        return (lambda: turn(q, k, pos, freq, scale=scale, sm_budget=a.sm_budget)), 0.0, 4.0 * S * B * (H + Hk) * d
+    if kernel in ("balance_fwd", "router_bwd"):     # M tokens, N experts, two choices each
+        from ..ops import moe as MOE
+        probs = torch.softmax(torch.randn(M, Nn, device="cuda"), -1)
+        top, ids = probs.topk(2, -1)
+        gates, dg = top / top.sum(-1, keepdim=True), torch.randn(M, 2, device="cuda")
+        if kernel == "balance_fwd":
+            return (lambda: MOE.balance_loss_fwd(probs, ids, sm_budget=a.sm_budget)), 0.0, 4.0 * M * Nn + 16.0 * M
+        bal = MOE.balance_loss_fwd(probs, ids)[2]
+        return (lambda: MOE.router_topk_bwd(dg, probs, ids, gates, Nn, 0.01, balance=bal, sm_budget=a.sm_budget)), 0.0, 8.0 * M * Nn + 32.0 * M
+    if kernel in ("distill_fwd", "distill_bwd"):    # M rows of N logits, 64 entries of a teacher each
+        lg = bf(M, Nn, scale=3.0)
+        lab = torch.randint(0, Nn, (M,), dtype=torch.int32, device="cuda")
+        ids, top = torch.randint(0, Nn, (M, 64), dtype=torch.int32, device="cuda"), bf(M, 64, scale=3.0)
+        if kernel == "distill_fwd":
+            return (lambda: L.vocab_parallel_distill_fwd(lg, lab, ids, top, 2.0, sm_budget=a.sm_budget)), 0.0, 2.0 * M * Nn
+        saved = L.vocab_parallel_distill_fwd(lg, lab, ids, top, 2.0)[2]
+        g, out = torch.full((M,), 1.0 / M, device="cuda"), torch.empty_like(lg)
+        return (lambda: L.vocab_parallel_distill_bwd_(lg, lab, ids, top, saved, g, g, 2.0, out=out, sm_budget=a.sm_budget)), 0.0, 4.0 * M * Nn
     raise SystemExit(f"unknown kernel {kernel}")
 
 

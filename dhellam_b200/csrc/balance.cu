@@ -339,8 +339,8 @@ struct BalCall {
 };
 
 static int bal_refuse(const char* what, const BalCall& c) {
-  if (c.T >= 0 && c.E > 0 && c.E <= B_MAX_E && c.k > 0 && c.k <= B_MAX_K && c.T * c.k < INT32_MAX) return 0;
-  set_last_error_c(what, "1 to 1024 experts, 1 to 32 choices, fewer than 2^31 choices in all");
+  if (c.T >= 0 && c.E > 0 && c.E <= B_MAX_E && c.k > 0 && c.k <= B_MAX_K && c.T * c.k <= (1 << 30)) return 0;
+  set_last_error_c(what, "1 to 1024 experts, 1 to 32 choices, at most 2^30 choices in all");
   return (int)cudaErrorInvalidValue;
 }
 static int bal_rc(const char* what, cudaError_t e) {

@@ -242,6 +242,24 @@ def test_balance_on_another_stream_in_a_graph_and_with_a_budget():
     check_balance(probs, ids, gates, dg, mask, sm_budget=5)
 
 
+def test_balance_of_many_clusters_in_a_graph_and_on_two_streams_at_once():
+    """The form whose last kernel is put in place before its predecessor ends, captured; two calls that run side by side."""
+    cases = [router_case(9000, 70, 3, seed=s, device=DEV) for s in (1, 2)]
+
+    def step(c, **kw):
+        probs, ids, gates, dg, mask = c
+        loss, counts, bal = M.balance_loss_fwd(probs, ids, mask, **kw)
+        return loss, counts, M.router_topk_bwd(dg, probs, ids, gates, 70, 0.1, balance=bal, **kw)
+    want = [step(c) for c in cases]
+    assert all(torch.equal(a, b) for a, b in zip(want[0], replay(lambda: step(cases[0]))))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = [step(c, stream=s) for c, s in zip(cases, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+
+
 def test_balance_of_differentiated_probabilities_stays_differentiable():
     probs, ids, gates, dg, _ = router_case(20, 6, 2, device=DEV)
     p = probs.clone().requires_grad_(True)
@@ -375,6 +393,34 @@ def test_distill_many_rows_are_the_same_whatever_shares_the_gpu_with_them():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(want, got))
     assert all(torch.equal(a, b) for a, b in zip(want, replay(lambda: run_distill(case, 2.5))))
+
+
+@pytest.mark.parametrize("K", [40, 700])
+def test_distill_few_rows_in_a_graph_and_on_two_streams_at_once(K):
+    """Rows that clusters of CTAs share; more entries than a CTA has threads."""
+    cases = [on_gpu(distill_case(7, 50000 + 3 * s, K, seed=s, dtype=BF)) for s in (1, 2)]
+    want = [run_distill(c, 1.7) for c in cases]
+    check_distill(distill_case(7, 50003, K, seed=1, dtype=BF), 1.7, *want[0], BF)
+    assert all(torch.equal(a, b) for a, b in zip(want[0], replay(lambda: run_distill(cases[0], 1.7))))
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = [run_distill(c, 1.7, stream=s) for c, s in zip(cases, streams)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
+
+
+def test_distill_all_entries_the_same_id():
+    """Every entry of a row, and its label, at one id; ids that share a slot of the table."""
+    T, V, K = 6, 70000, 300
+    z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, seed=3, dtype=F32)
+    ids[0] = labels[0] = 65
+    ids[1] = torch.arange(K) * 227 % V
+    ids[2] = (torch.arange(K) % 7) * 4096
+    ids[3, ::2] = labels[3] = 12345
+    case = (z, labels, ids, top, g_ce, g_kd)
+    for tau in (1.0, 2.6):
+        check_distill(case, tau, *run_distill(on_gpu(case), tau), F32)
 
 
 def test_distill_far_rows_of_a_long_batch():
