@@ -610,10 +610,11 @@ struct DistillCall {
 };
 
 static int d_refuse(const char* what, const DistillCall& c) {
-  if (c.T >= 0 && c.T <= INT32_MAX && c.Vl > 0 && c.K >= 0 && c.K <= D_MAX_K && c.v0 >= 0 && c.V >= c.v0 + c.Vl && c.V <= INT32_MAX &&
+  // 2^30: a row's or an element's number plus one step of a loop stays in 31 bits
+  if (c.T >= 0 && c.T <= (1 << 30) && c.Vl > 0 && c.Vl <= (1 << 30) && c.K >= 0 && c.K <= D_MAX_K && c.v0 >= 0 && c.V >= c.v0 + c.Vl && c.V <= INT32_MAX &&
       c.tau > 0. && 1. / c.tau <= FLT_MAX && (float)c.tau > 0.f && (float)c.tau <= FLT_MAX)
     return 0;
-  set_last_error_c(what, "a shard inside a vocabulary of at most 2^31 - 1 entries, at most 1024 teacher's entries, a positive temperature");
+  set_last_error_c(what, "a shard inside a vocabulary of at most 2^31 - 1 entries, at most 2^30 rows and entries a shard, 1024 teacher's entries, a positive temperature");
   return (int)cudaErrorInvalidValue;
 }
 static int d_rc(const char* what, cudaError_t e) {

@@ -209,9 +209,9 @@ int dh_rope_heads(const void* call) {
   const int64_t rows = c.rows, inner = c.inner;
   const int heads_q = (int)c.heads_q, heads_k = (int)c.heads_k, d = (int)c.d, rotated = (int)c.rotated;
   const int64_t* ptrs = c.ptrs;
-  if (c.heads_q < 0 || c.heads_k < 0 || c.heads_q + c.heads_k > INT32_MAX || c.d <= 0 || c.d > 65536 || c.rotated <= 0 || c.rotated > c.d ||
+  if (c.heads_q < 0 || c.heads_k < 0 || c.heads_q > (1 << 29) || c.heads_k > (1 << 29) || c.d <= 0 || c.d > 65536 || c.rotated <= 0 || c.rotated > c.d ||
       (c.rotated & 1) || rows < 0 || inner <= 0 || inner > INT32_MAX) {
-    set_last_error_c("dh_rope_heads", "sizes out of range (an even number of rotated elements, at most the head size)");
+    set_last_error_c("dh_rope_heads", "sizes out of range (an even number of rotated elements, at most the head size; at most 2^29 heads each)");
     return (int)cudaErrorInvalidValue;
   }
   if (rows == 0 || heads_q + heads_k == 0) return 0;

@@ -65,14 +65,20 @@ def use_library(t) -> bool:
 def is_plain(t) -> bool:
     """True for an ordinary tensor of the current device that nobody differentiates, traces or maps over: a kernel may
     stand in for the PyTorch ops on it.  (Ops that have never been composed of PyTorch ops need no such question.)"""
-    return are_plain(t)
+    return t is not None and are_plain(t)
 
 
 def are_plain(*tensors) -> bool:
     """``is_plain`` of every tensor (``None`` is skipped)."""
-    device, grad = torch._C._cuda_getDevice() if _LIB is not None or available() else -1, torch.is_grad_enabled()
+    device, grad = -1, torch.is_grad_enabled()
     for t in tensors:
-        if t is not None and not (type(t) is torch.Tensor and t.is_cuda and t.get_device() == device and not (grad and t.requires_grad)):
+        if t is None:
+            continue
+        if type(t) is not torch.Tensor or not t.is_cuda or (grad and t.requires_grad):
+            return False
+        if device < 0:                   # asked for a CUDA tensor alone: without a GPU the question is an error
+            device = torch._C._cuda_getDevice()
+        if t.get_device() != device:
             return False
     return forward_ad._current_level < 0 and torch._C._functorch.peek_interpreter_stack() is None \
         and torch._C._len_torch_dispatch_stack() == 0 and not torch.jit.is_tracing() and not torch.compiler.is_compiling()

@@ -61,8 +61,8 @@ def _router_operands(what, probs, topi, mask):
 def _on_kernel(probs, topi, *others):
     """Whether the kernels of csrc/balance.cu take these operands.  Both functions were composed of PyTorch ops before and still are for
     what only those handle: CPU tensors, the library backend, tensors that are differentiated, traced or on another device, more than
-    1024 experts or 32 choices."""
-    return K.use_native(probs) and probs.shape[1] <= 1024 and topi.shape[1] <= 32 and (probs.stride(1) == 1 or probs.shape[1] == 1) \
+    1024 experts or 32 choices, more than 2^30 choices in all."""
+    return K.use_native(probs) and 0 < probs.shape[1] <= 1024 and topi.shape[1] <= 32 and topi.numel() <= 1 << 30 and (probs.stride(1) == 1 or probs.shape[1] == 1) \
         and K.are_plain(probs, topi, *others)
 
 
@@ -78,6 +78,17 @@ def _router_call(probs, topi, mask, sm_budget):
     return _ROUTER_CALL.pack(probs.data_ptr(), probs.stride()[0], topi.data_ptr(), topi.stride()[0], topi.dtype is torch.int64,
                              mask.data_ptr() if mask is not None else 0, T, E, topi.shape[1], sm_budget,
                              torch._C._cuda_getCurrentRawStream(probs.get_device()))
+
+
+def _balance_coef(topi, E, mask):
+    """``(counted [T] bool, counts [E] int64, coef [E] fp32)`` of PyTorch ops that ask the host nothing."""
+    T, k = topi.shape
+    counted = torch.ones(T, dtype=torch.bool, device=topi.device) if mask is None else mask != 0
+    n = counted.sum().clamp_min(1)
+    # an extra column takes the choices that count for nobody
+    used = torch.where((topi >= 0) & (topi < E) & counted[:, None], topi.long(), E).reshape(-1)
+    counts = torch.zeros(E + 1, dtype=torch.int64, device=topi.device).index_add_(0, used, torch.ones_like(used))[:E]
+    return counted, counts, counts.to(torch.float32) / n / n * (E / max(k, 1))
 
 
 def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
@@ -102,12 +113,7 @@ def balance_loss_fwd(probs, topi, mask=None, sm_budget: int = 0, stream=None):
         scratch = probs.new_empty(words) if words else None
         K.check(K.proto("dh_balance_fwd", _BALANCE_FWD)(call, K.ptr(scratch), loss.data_ptr(), counts.data_ptr(), coef.data_ptr()), "dh_balance_fwd")
         return loss, counts, Balance(coef, mask)
-    counted = torch.ones(T, dtype=torch.bool, device=probs.device) if mask is None else mask != 0
-    n = counted.sum().clamp_min(1)
-    # an extra column takes the choices that count for nobody
-    used = torch.where((topi >= 0) & (topi < E) & counted[:, None], topi.long(), E).reshape(-1)
-    counts = torch.bincount(used, minlength=E + 1)[:E]
-    coef = counts.to(torch.float32) / n / n * (E / k)
+    counted, counts, coef = _balance_coef(topi, E, mask)
     loss = (coef * torch.where(counted[:, None], probs, torch.zeros_like(probs)).sum(0)).sum()
     return loss, counts.to(torch.int32), Balance(coef, mask)
 
@@ -127,14 +133,18 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
     if stream is not None:
         operands = (d_gates, probs, topi, gates) + (tuple(balance) if balance is not None else ())
         return K.run_on_stream(stream, operands, lambda: router_topk_bwd(d_gates, probs, topi, gates, E, aux_scale, balance, sm_budget))
-    mask = balance.mask if balance is not None else None
-    _router_operands("router_topk_bwd", probs, topi, mask)
-    if probs.shape[1] != E or d_gates.shape != topi.shape or gates.shape != topi.shape or (balance is not None and balance.coef.shape != (E,)):
-        raise ValueError(f"router_topk_bwd: gates and their gradient as the choices {tuple(topi.shape)}, probabilities and balance of {E} "
-                         f"experts")
+    coef, mask = balance if balance is not None else (None, None)
     T, k = topi.shape
-    coef = balance.coef if balance is not None else None
-    if _on_kernel(probs, topi, d_gates, gates, mask, coef) and d_gates.dtype is gates.dtype is torch.float32 \
+    if probs.shape != (T, E) or d_gates.shape != topi.shape or gates.shape != topi.shape:
+        raise ValueError(f"router_topk_bwd: gates and their gradient as the choices {tuple(topi.shape)}, as many rows of {E} "
+                         f"probabilities, got {tuple(gates.shape)}, {tuple(d_gates.shape)} and {tuple(probs.shape)}")
+    if balance is not None:
+        _router_operands("router_topk_bwd", probs, topi, mask)
+        if coef.shape != (E,):
+            raise ValueError(f"router_topk_bwd: a balance of {E} experts, got {tuple(coef.shape)}")
+    # fp64 probabilities, a weight in a tensor and the like were taken before there was a kernel, and still are by the ops below
+    if k > 0 and probs.dtype is d_gates.dtype is gates.dtype is torch.float32 and topi.dtype in (torch.int32, torch.int64) \
+            and isinstance(aux_scale, (int, float)) and _on_kernel(probs, topi, d_gates, gates, mask, coef) \
             and (coef is None or coef.dtype is torch.float32):
         if aux_scale and coef is None:
             coef = balance_loss_fwd(probs, topi)[2].coef
@@ -158,7 +168,7 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
     d_probs = torch.zeros_like(probs)
     d_probs.scatter_add_(1, at, d_topv)
     if aux_scale:
-        d_aux = aux_scale * (balance_loss_fwd(probs, topi)[2].coef if coef is None else coef)[None, :]
+        d_aux = aux_scale * (_balance_coef(topi, E, None)[2] if coef is None else coef)[None, :]
         if mask is not None:
             d_aux = torch.where(mask[:, None] != 0, d_aux, torch.zeros_like(d_aux))
         d_probs = d_probs + d_aux

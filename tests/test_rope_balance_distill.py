@@ -287,3 +287,45 @@ def _two_shards(rank, world):
 def test_distill_over_two_vocabulary_shards():
     from dist_utils import run_ranks
     run_ranks(_two_shards, 2)
+
+
+def test_router_gradient_takes_what_it_took_before():
+    """Probabilities in 64 bits, a weight in a tensor, no balance: PyTorch's ops by their types, against the formula."""
+    probs, topi, gates, dg = (t.double() if t.is_floating_point() else t for t in router_case(50, 7, 3, 5)[:4])
+    topi = topi.long()
+    for weight in (0.0, 0.25, torch.tensor(0.25)):
+        got = M.router_topk_bwd(dg, probs, topi, gates, 7, weight)
+        p = probs.clone()
+        d = torch.zeros_like(p).scatter_add(1, topi, (dg - (dg * gates).sum(1, keepdim=True)) / p.gather(1, topi).sum(1, keepdim=True))
+        d = d + float(weight) * 7 * torch.bincount(topi.reshape(-1), minlength=7).double() / topi.numel() / 50
+        want = p * (d - (d * p).sum(1, keepdim=True))
+        # the balance's coefficients are fp32 numbers of three roundings
+        assert got.dtype == torch.float64 and float((got - want).abs().max()) <= 1e-12 + 4 * 2.0 ** -24 * 0.25 * 7
+
+
+def test_questions_about_tensors_need_no_gpu():
+    """With the library loaded, where there may be no GPU: a CPU tensor and nothing at all are no operands of a kernel."""
+    from ctypes import c_int, c_void_p
+    from dhellam_b200 import kernels as K
+    K.proto("dh_distill_combine", [c_void_p, c_int])
+    assert not K.is_plain(torch.ones(2)) and not K.are_plain(torch.ones(2)) and not K.is_plain(None) and not K.are_plain(None, torch.ones(2))
+
+
+def test_sizes_beyond_31_bits_of_a_loop_are_refused():
+    """By the C functions, before anything is launched (sizes alone: no such tensor is made)."""
+    from dhellam_b200 import kernels as K
+    from ctypes import c_float, c_int64, c_void_p
+    def call(name, types, *args):
+        return K.proto(name, types)(*args)
+    big = (1 << 30) + 1
+    for T, V in ((big, 4), (4, big)):
+        c = L._DISTILL_CALL.pack(0, V, 0, 0, 0, 0, 0, 0, 0, 0, T, V, 0, 0, 2 ** 31 - 1, 0, 0, 1.0)
+        assert call("dh_distill_fwd", L._DISTILL_FWD, c, 0, 0, 0, 0) != 0
+        assert call("dh_distill_bwd", L._DISTILL_BWD, c, 0, 0, 0, 0, V) != 0
+    for T, E, k in ((1 << 28, 8, 5), (8, 1025, 2), (8, 4, 33), (8, 0, 1)):
+        c = M._ROUTER_CALL.pack(0, E, 0, k, 0, 0, T, E, k, 0, 0)
+        assert call("dh_balance_fwd", M._BALANCE_FWD, c, 0, 0, 0, 0) != 0
+        assert call("dh_router_bwd", M._ROUTER_BWD, c, 0, k, 0, k, 0, 0.0, 0) != 0
+    for heads_q, heads_k in (((1 << 29) + 1, 1), (0, (1 << 29) + 1)):
+        c = R._ROPE_CALL.pack(*[0] * 16, heads_q, heads_k, 0, 0, 0, 1, 1, 2, 2, 0, 0, 0, 0, 0, 1.0)
+        assert call("dh_rope_heads", R._ROPE_ARGS, c) != 0

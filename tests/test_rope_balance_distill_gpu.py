@@ -260,6 +260,20 @@ def test_balance_of_many_clusters_in_a_graph_and_on_two_streams_at_once():
         assert all(torch.equal(a, b) for w, g in zip(want, got) for a, b in zip(w, g))
 
 
+def test_router_of_more_experts_than_the_kernel_takes_in_a_graph():
+    """PyTorch's ops for 1100 experts ask the host nothing, so they can be captured as before there was a kernel."""
+    probs, ids, gates, dg, mask = router_case(60, 1100, 4, device=DEV)
+    for balance in (False, True):
+        def step():
+            bal = M.balance_loss_fwd(probs, ids, mask)[2] if balance else None
+            return M.router_topk_bwd(dg, probs, ids, gates, 1100, 0.5, balance=bal)
+        want = step()
+        assert torch.equal(replay(step), want)
+        coef = O.balance(probs.cpu(), ids.cpu(), mask.cpu() if balance else None)[2]
+        exact, bound = O.router_gradient(dg.cpu(), probs.cpu(), ids.cpu(), gates.cpu(), 0.5, coef, mask.cpu() if balance else None)
+        assert bool(((want.cpu().double() - exact).abs() <= bound).all())
+
+
 def test_balance_of_differentiated_probabilities_stays_differentiable():
     probs, ids, gates, dg, _ = router_case(20, 6, 2, device=DEV)
     p = probs.clone().requires_grad_(True)
