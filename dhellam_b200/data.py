@@ -107,8 +107,8 @@ class TokenFileDataset:
             raise ValueError(f"{path}: {len(self.tokens)} tokens are fewer than one sample of {seq_length + 1}")
         self.seed = seed
         self._perm_epoch, self._perm = -1, None
-        if teacher is not None and teacher.n < len(self.tokens) - 1:
-            raise ValueError(f"{path}: {len(self.tokens)} tokens, but the teacher's entries of {teacher.n} positions")
+        if teacher is not None and teacher.n not in (len(self.tokens) - 1, len(self.tokens)):      # a wrong k may divide the file too
+            raise ValueError(f"{path}: {len(self.tokens)} tokens, but the teacher's entries, {teacher.k} each, of {teacher.n} positions")
         self.teacher = teacher
 
     def __len__(self):

@@ -122,9 +122,11 @@ def loss_fwd(env, hp: HeadParams, mb, x):
     if alpha:
         if mb.teacher_ids is None:
             raise ValueError("distillation (distill_alpha > 0) needs a teacher's top logits in every micro-batch")
-        ce, kd, lse = L.vocab_parallel_distill_fwd(logits, mb.labels, mb.teacher_ids, mb.teacher_logits, env.train.distill_temperature, v0,
-                                                   env.ps.tp_group)
-        loss_tok = (1.0 - alpha) * ce + alpha * kd
+        # without a share of the cross entropy it is not computed: nothing times infinitely much is no loss
+        ce, kd, lse = L.vocab_parallel_distill_fwd(logits, mb.labels if alpha < 1.0 else None, mb.teacher_ids, mb.teacher_logits,
+                                                   env.train.distill_temperature, v0, env.ps.tp_group)
+        loss_tok = (1.0 - alpha) * ce + alpha * kd if alpha < 1.0 else kd
+        loss_tok = torch.where(mb.loss_mask.reshape(-1) != 0, loss_tok, 0.0)      # whatever the teacher says about padding
     else:
         loss_tok, lse = L.vocab_parallel_ce_fwd(logits, mb.labels, v0, env.ps.tp_group, label_smoothing=env.train.label_smoothing)
     mask = mb.loss_mask.reshape(-1).float()
@@ -143,8 +145,9 @@ def loss_bwd(env, hp: HeadParams, mb, saved, grad_scale: float):
     logits = _use(env, saved.pop("logits"))
     alpha, stat = env.train.distill_alpha, _use(env, saved.pop("lse"))
     if alpha:
-        dlogits = L.vocab_parallel_distill_bwd_(logits, mb.labels, mb.teacher_ids, mb.teacher_logits, stat, (1.0 - alpha) * g_tok,
-                                                alpha * g_tok, env.train.distill_temperature, v0)
+        labels, g_ce = (mb.labels, (1.0 - alpha) * g_tok) if alpha < 1.0 else (None, None)
+        dlogits = L.vocab_parallel_distill_bwd_(logits, labels, mb.teacher_ids, mb.teacher_logits, stat, g_ce, alpha * g_tok,
+                                                env.train.distill_temperature, v0)
     else:
         dlogits = L.vocab_parallel_ce_bwd_(logits, mb.labels, stat, g_tok, v0, label_smoothing=env.train.label_smoothing,
                                            vocab=env.cfg.vocab_size)

@@ -234,6 +234,48 @@ def test_arguments_reach_the_configuration():
     assert (cfg.rope_scaling, cfg.rope_scaling_factor) == ("linear", 4.0)
 
 
+def test_a_teachers_entries_of_padding_do_not_matter():
+    """Rows that the loss leaves out: NaN and infinities among the teacher's logits there change neither the loss nor a gradient."""
+    from dhellam_b200.config import ParallelConfig, TrainConfig, preset
+    from dhellam_b200.data import synthetic_step_batches
+    from dhellam_b200.parallel import state as PS
+    from dhellam_b200.trainer import Trainer
+    cfg = preset("tiny-llama", seq_length=16)
+    for alpha in (0.5, 1.0):
+        train = TrainConfig(micro_batch_size=2, global_batch_size=2, dtype="fp32", distill_alpha=alpha, distill_temperature=2.0)
+        got = []
+        for poison in (False, True):
+            PS.set_state(None)
+            tr = Trainer(cfg, ParallelConfig(), train, device="cpu")
+            mbs = synthetic_step_batches(cfg, train, tr.ps, 0, "cpu")
+            left_out = torch.arange(32) % 5 == 0
+            mbs[0].loss_mask.view(-1)[left_out] = 0
+            if poison:
+                mbs[0].teacher_logits[left_out] = torch.tensor([math.nan, math.inf] * 8, dtype=torch.float16)
+            else:
+                mbs[0].teacher_ids[left_out] = -1
+            tr.optimizer.zero_grad()
+            losses = tr.engine.run_step(mbs)
+            got.append((losses[0], tr.model.dchb.word_embeddings.main_grad.clone()))
+        assert math.isfinite(float(got[0][0])) and torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_a_teacher_file_of_other_rows_or_without_tokens_is_refused(tmp_path):
+    import os
+    import subprocess
+    import sys
+    import numpy as np
+    from dhellam_b200.data import TeacherTopFile, TokenFileDataset
+    from test_train_cli import ARGS, ROOT
+    np.arange(100, dtype=np.int32).tofile(str(tmp_path / "t.bin"))
+    _write_teacher(str(tmp_path / "top"), 100, 6, 50)
+    with pytest.raises(ValueError, match="200 positions"):          # three entries a row divide the file as well
+        TokenFileDataset(str(tmp_path / "t.bin"), 20, teacher=TeacherTopFile(str(tmp_path / "top"), 3))
+    p = subprocess.run([sys.executable, os.path.join(ROOT, "train.py")] + ARGS + ["--train-iters", "1", "--distill-alpha", "0.5", "--distill-data",
+                       str(tmp_path / "top")], cwd=str(tmp_path), env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=300)
+    assert p.returncode != 0 and "--data-path" in p.stderr
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("alpha,tau", [(0.0, 1.0), (0.5, 2.0), (0.7, 1.5)])
 @pytest.mark.parametrize("family", ["llama", "moe"])

@@ -64,6 +64,8 @@ def main(argv=None):
                 f"{train.num_microbatches(pcfg.dp)} micro-batches of {train.micro_batch_size} per step, "
                 f"dual-strand {'on' if train.dhellam else 'off'}, fused comm {'on' if tr.env.fused_tp else 'off'}")
     dataset = None
+    if args.distill_data and (args.mock_data or not args.data_path):
+        raise ValueError("--distill-data holds a teacher's entries of the tokens in --data-path, which is not given")
     if args.data_path and not args.mock_data:
         # a flat token file (the payload of a Megatron .bin file); "<path>:<dtype>" selects the id type
         path, _, dt = args.data_path[-1].partition(":")
