@@ -10,7 +10,7 @@
 // by 0.03 rad at position 10^6).
 //
 // One thread holds the cosines and sines of V pairs of one row in registers and walks over heads with them, several in flight: two 16-byte
-// loads and stores per head.  Bound by memory: 65536 x 40 heads of 128, 217 us (6.2 TB/s).  A table of a CTA's angles in shared memory, so
+// loads and stores per head.  Bound by memory: 65536 x 40 heads of 128, 214 us (6.3 TB/s).  A table of a CTA's angles in shared memory, so
 // that threads that share a row do not compute them anew, was slower (225 us; 65536 x 3 heads 39 against 27), and so was one head at a
 // time (243 us).
 //
@@ -256,12 +256,15 @@ int dh_rope_heads(const void* call) {
   // threads that share the heads of a row: enough of them to fill half of the GPU's threads, where there are that few rows
   a.groups = 1;
   while (a.groups * 2 <= heads_q + heads_k && rows * a.units * a.groups < (int64_t)budget * 1024) a.groups *= 2;
+  // CTAs of a launch; beyond them they walk on.  On the whole GPU 8, 16, 32 per SM and as many as there are: 200000 x 40 heads of 128 661,
+  // 637, 631 and 632 us, 500000 x 3 155, 153, 152 and 160 us.
+  const int64_t cap = (int64_t)budget * (budget < sms ? 8 : 32);
   const int64_t most = INT32_MAX / ((int64_t)a.units * a.groups);      // rows of one launch: item numbers stay in 31 bits
   for (int64_t r = 0; r < rows; r += most) {
     a.row0 = r;
     a.rows = rows - r < most ? rows - r : most;
     const int64_t blocks = (a.rows * a.units * a.groups + RT - 1) / RT;
-    const int grid = (int)(blocks < (int64_t)budget * 8 ? blocks : (int64_t)budget * 8);
+    const int grid = (int)(blocks < cap ? blocks : cap);
     if (c.f32) {
       if (V == 4) rope_launch<float, 4>(a, interleaved, grid, s);
       else if (V == 2) rope_launch<float, 2>(a, interleaved, grid, s);
