@@ -15,7 +15,7 @@
 // time (243 us).
 //
 // Interleaved, a vector may hold pairs that are turned and pairs that stay, so V follows from addresses and strides alone.  In halves it has
-// to divide half the rotated elements too (16384 x 80 heads of 96, 38 rotated: 93 us interleaved, 224 us in halves, element by element).
+// to divide half the rotated elements too; where that leaves little of a vector, whole heads pass through shared memory (second kernel).
 // Elements that are only copied stay with the pairs of their head: as work items behind all pairs they tore the lines of memory apart
 // (3799 x 80 heads of 128, 64 rotated: 37 against 51 us).
 #include <cuda_bf16.h>
@@ -84,6 +84,12 @@ __device__ __forceinline__ RopeRaw<T, V> rope_pack(const float (&f)[V]) {
   }
   return r;
 }
+// One pair, the same bits wherever it is turned: the results of a row do not depend on what shares the call with it.
+__device__ __forceinline__ void rope_pair(float& x, float& y, float c, float s) {
+  const float u = __fmul_rn(y, s), w = __fmul_rn(x, s);
+  x = fmaf(x, c, -u);
+  y = fmaf(y, c, w);
+}
 // Turns V pairs: x the first, y the second elements; interleaved, x has the first V/2 pairs, y the others, and those from n on stay.
 template <typename T, int V, bool INTERLEAVED>
 __device__ __forceinline__ void rope_turn(RopeRaw<T, V>& x, RopeRaw<T, V>& y, const float (&cs)[V], const float (&sn)[V], int n) {
@@ -94,17 +100,12 @@ __device__ __forceinline__ void rope_turn(RopeRaw<T, V>& x, RopeRaw<T, V>& y, co
 #pragma unroll
     for (int j = 0; j < V; j += 2) {
       const int f = j / 2, s = V / 2 + j / 2;
-      const float p0 = p[j], q0 = q[j];
-      if (f < n) { p[j] = p0 * cs[f] - p[j + 1] * sn[f]; p[j + 1] = p[j + 1] * cs[f] + p0 * sn[f]; }
-      if (s < n) { q[j] = q0 * cs[s] - q[j + 1] * sn[s]; q[j + 1] = q[j + 1] * cs[s] + q0 * sn[s]; }
+      if (f < n) rope_pair(p[j], p[j + 1], cs[f], sn[f]);
+      if (s < n) rope_pair(q[j], q[j + 1], cs[s], sn[s]);
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float p0 = p[j];
-      p[j] = p0 * cs[j] - q[j] * sn[j];
-      q[j] = q[j] * cs[j] + p0 * sn[j];
-    }
+    for (int j = 0; j < V; ++j) rope_pair(p[j], q[j], cs[j], sn[j]);
   }
   RopeRaw<T, V> rx = rope_pack<T, V>(p), ry = rope_pack<T, V>(q);
   if constexpr (INTERLEAVED && V > 1 && sizeof(T) == 2) {       // what stays, stays bit by bit: a NaN's bits do not survive the conversion
@@ -184,6 +185,120 @@ __global__ void __launch_bounds__(RT, 3) rope_heads_kernel(const RopeArgs a) {
   }
 }
 
+// Pairs in halves whose half is an odd number of elements, or of pairs of bf16: a warp brings whole heads of a row into shared memory by
+// vectors, turns them there, W pairs of a lane side by side, and sends them out by vectors.  Where half a head's pairs need 16 lanes or
+// fewer, 2, 4, ... heads are turned at a time.  NP: times that a lane has W pairs of a head.  Bound by the instructions around the
+// vectors: the addresses of a row's heads are kept over its steps (16384 x 80 heads of 96, 38 rotated: 109 -> 92 us), and the next
+// step's vectors are asked for before this one's are turned (114 -> 109 us).  Three CTAs per SM: with four a few registers spill, 158 us.
+constexpr int RS = 4;                         // vectors of a lane at a time: 2 KB a warp
+template <typename T, int W> struct RopeWords;
+template <> struct RopeWords<float, 1> {
+  using type = float;
+  __device__ static __forceinline__ void get(float w, float (&f)[1]) { f[0] = w; }
+  __device__ static __forceinline__ float put(const float (&f)[1]) { return f[0]; }
+};
+template <> struct RopeWords<__nv_bfloat16, 1> {
+  using type = __nv_bfloat16;
+  __device__ static __forceinline__ void get(__nv_bfloat16 w, float (&f)[1]) { f[0] = __bfloat162float(w); }
+  __device__ static __forceinline__ __nv_bfloat16 put(const float (&f)[1]) { return __float2bfloat16(f[0]); }
+};
+template <> struct RopeWords<__nv_bfloat16, 2> {
+  using type = uint32_t;
+  __device__ static __forceinline__ void get(uint32_t w, float (&f)[2]) { const float2 p = unpack_bf16x2(w); f[0] = p.x; f[1] = p.y; }
+  __device__ static __forceinline__ uint32_t put(const float (&f)[2]) { return pack_bf16x2(f[0], f[1]); }
+};
+
+template <typename T, int W, int LANES, int NP>
+__global__ void __launch_bounds__(RT, 3) rope_staged_kernel(const RopeArgs a) {
+  constexpr int BATCH = 4 / W, SUBS = 32 / LANES;         // heads of a lane at a time, lanes' groups
+  using Words = RopeWords<T, W>;
+  using Word = typename Words::type;
+  __shared__ uint4 stage[RT / 32][RS * 32];
+  const int lane = threadIdx.x & 31, sub = lane / LANES, li = lane % LANES;
+  uint4* const mine = stage[threadIdx.x >> 5];
+  const int vecs = a.units, per = RS * 32 / vecs, all = a.heads[0] + a.heads[1];      // vectors of a head, heads of a step
+  int head[RS];
+#pragma unroll
+  for (int s = 0; s < RS; ++s) head[s] = min((s * 32 + lane) / vecs, per);
+  const auto offset = [&](int s) { return s * 32 + lane - head[s] * vecs; };
+  const auto there = [&](int s, int first) { return head[s] < per && first + head[s] < all; };
+  const unsigned int total = (unsigned int)(a.rows * a.groups), step = gridDim.x * (RT / 32);
+  for (unsigned int i = blockIdx.x * (RT / 32) + (threadIdx.x >> 5); i < total; i += step) {
+    const unsigned int r = i / a.groups, group = i - r * a.groups;
+    const long long row = a.row0 + r;
+    const long long outer = row / a.inner, inner = row - outer * a.inner;
+    const T* const in0 = reinterpret_cast<const T*>(a.t[0].in) + outer * a.t[0].is0 + inner * a.t[0].is1;
+    const T* const in1 = reinterpret_cast<const T*>(a.t[1].in) + outer * a.t[1].is0 + inner * a.t[1].is1 - a.heads[0] * a.t[1].ish;
+    T* const out0 = reinterpret_cast<T*>(a.t[0].out) + outer * a.t[0].os0 + inner * a.t[0].os1;
+    T* const out1 = reinterpret_cast<T*>(a.t[1].out) + outer * a.t[1].os0 + inner * a.t[1].os1 - a.heads[0] * a.t[1].osh;
+    uint4 v[RS];
+    const auto fetch = [&](int first) {
+#pragma unroll
+      for (int s = 0; s < RS; ++s) {
+        const int h = first + head[s];
+        if (!there(s, first)) continue;
+        const T* src = h < a.heads[0] ? in0 + h * a.t[0].ish : in1 + h * a.t[1].ish;
+        v[s] = reinterpret_cast<const uint4*>(src)[offset(s)];
+      }
+    };
+    fetch((int)group * per);
+    const double p = a.pos64 ? (double)reinterpret_cast<const long long*>(a.pos)[row] : (double)reinterpret_cast<const int*>(a.pos)[row];
+    float cs[NP][W], sn[NP][W];
+#pragma unroll
+    for (int j = 0; j < NP; ++j)
+#pragma unroll
+      for (int q = 0; q < W; ++q) {
+        const double turns = p * a.freq[min((li + LANES * j) * W + q, a.half - 1)] * 0.15915494309189533577;
+        float s, k;
+        sincospif((float)(2.0 * (turns - rint(turns))), &s, &k);
+        cs[j][q] = k * a.scale;
+        sn[j][q] = s * a.scale * a.sign;
+      }
+    for (int first = (int)group * per; first < all; first += a.groups * per) {
+#pragma unroll
+      for (int s = 0; s < RS; ++s)
+        if (there(s, first)) mine[s * 32 + lane] = v[s];
+      fetch(first + a.groups * per);
+      __syncwarp();
+      const int count = min(per, all - first);
+      for (int g = sub; g < count; g += BATCH * SUBS) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          if ((li + LANES * j) * W >= a.half) continue;
+          T* const e = reinterpret_cast<T*>(mine) + g * a.d + (li + LANES * j) * W;
+          Word x[BATCH], y[BATCH];
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u)
+            if (g + u * SUBS < count) {
+              x[u] = *reinterpret_cast<const Word*>(e + u * SUBS * a.d);
+              y[u] = *reinterpret_cast<const Word*>(e + u * SUBS * a.d + a.half);
+            }
+#pragma unroll
+          for (int u = 0; u < BATCH; ++u)
+            if (g + u * SUBS < count) {
+              float f[W], t[W];
+              Words::get(x[u], f);
+              Words::get(y[u], t);
+#pragma unroll
+              for (int q = 0; q < W; ++q) rope_pair(f[q], t[q], cs[j][q], sn[j][q]);
+              *reinterpret_cast<Word*>(e + u * SUBS * a.d) = Words::put(f);
+              *reinterpret_cast<Word*>(e + u * SUBS * a.d + a.half) = Words::put(t);
+            }
+        }
+      }
+      __syncwarp();
+#pragma unroll
+      for (int s = 0; s < RS; ++s) {
+        const int h = first + head[s];
+        if (!there(s, first)) continue;
+        T* dst = h < a.heads[0] ? out0 + h * a.t[0].osh : out1 + h * a.t[1].osh;
+        reinterpret_cast<uint4*>(dst)[offset(s)] = mine[s * 32 + lane];
+      }
+      __syncwarp();
+    }
+  }
+}
+
 // All fields 8 bytes wide, as the Python layer packs them.  ptrs: q in, q out, k in, k out; strides (elements): for each of them the outer
 // row, inner row and head stride; rows are outer x inner.
 struct RopeCall {
@@ -195,6 +310,20 @@ template <typename T, int V>
 static void rope_launch(const RopeArgs& a, int interleaved, int grid, cudaStream_t s) {
   if (interleaved) rope_heads_kernel<T, V, true><<<grid, RT, 0, s>>>(a);
   else rope_heads_kernel<T, V, false><<<grid, RT, 0, s>>>(a);
+}
+
+template <typename T, int W>
+static void rope_launch_staged(const RopeArgs& a, int words, int grid, cudaStream_t s) {
+  if (words <= 8) rope_staged_kernel<T, W, 8, 1><<<grid, RT, 0, s>>>(a);
+  else if (words <= 16) rope_staged_kernel<T, W, 16, 1><<<grid, RT, 0, s>>>(a);
+  else if (words <= 32) rope_staged_kernel<T, W, 32, 1><<<grid, RT, 0, s>>>(a);
+  else if (words <= 64) rope_staged_kernel<T, W, 32, 2><<<grid, RT, 0, s>>>(a);
+  else rope_staged_kernel<T, W, 32, 4><<<grid, RT, 0, s>>>(a);
+}
+static int rope_rc() {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) set_last_error_c("dh_rope_heads", cudaGetErrorString(e));
+  return (int)e;
 }
 
 }  // namespace dh
@@ -209,9 +338,9 @@ int dh_rope_heads(const void* call) {
   const int64_t rows = c.rows, inner = c.inner;
   const int heads_q = (int)c.heads_q, heads_k = (int)c.heads_k, d = (int)c.d, rotated = (int)c.rotated;
   const int64_t* ptrs = c.ptrs;
-  if (c.heads_q < 0 || c.heads_k < 0 || c.heads_q > (1 << 29) || c.heads_k > (1 << 29) || c.d <= 0 || c.d > 65536 || c.rotated <= 0 || c.rotated > c.d ||
+  if (c.heads_q < 0 || c.heads_k < 0 || c.heads_q > (1 << 28) || c.heads_k > (1 << 28) || c.d <= 0 || c.d > 65536 || c.rotated <= 0 || c.rotated > c.d ||
       (c.rotated & 1) || rows < 0 || inner <= 0 || inner > INT32_MAX) {
-    set_last_error_c("dh_rope_heads", "sizes out of range (an even number of rotated elements, at most the head size; at most 2^29 heads each)");
+    set_last_error_c("dh_rope_heads", "sizes out of range (an even number of rotated elements, at most the head size; at most 2^28 heads each)");
     return (int)cudaErrorInvalidValue;
   }
   if (rows == 0 || heads_q + heads_k == 0) return 0;
@@ -219,13 +348,13 @@ int dh_rope_heads(const void* call) {
   const bool in_place = (heads_q == 0 || ptrs[0] == ptrs[1]) && (heads_k == 0 || ptrs[2] == ptrs[3]);
   const int interleaved = (int)c.interleaved;
   // the widest vector that divides every address and stride, and a head (interleaved) or half the rotated part and the rest (in halves)
-  uint64_t odd = (uint64_t)(interleaved ? d : rotated / 2) * size;
-  if (!interleaved && !in_place) odd |= (uint64_t)(d - rotated) * size;
+  uint64_t wide = 0;
   for (int i = 0; i < 4; ++i) {
     if ((i < 2 ? heads_q : heads_k) == 0) continue;
-    odd |= (uint64_t)ptrs[i];
-    for (int j = 0; j < 3; ++j) odd |= (uint64_t)(c.strides[3 * i + j] * size);
+    wide |= (uint64_t)ptrs[i];
+    for (int j = 0; j < 3; ++j) wide |= (uint64_t)(c.strides[3 * i + j] * size);
   }
+  const uint64_t odd = wide | (uint64_t)(interleaved ? d : rotated / 2) * size | (interleaved || in_place ? 0 : (uint64_t)(d - rotated) * size);
   const int bytes = (odd & 15) == 0 ? 16 : (odd & 7) == 0 ? 8 : (odd & 3) == 0 ? 4 : 2;
   const int V = bytes / size;
   if (V == 0) {
@@ -247,18 +376,41 @@ int dh_rope_heads(const void* call) {
   a.inner = (int)inner;
   a.half = rotated / 2;
   a.d = d;
-  a.rot_units = (a.half + V - 1) / V;
-  const int rest = interleaved ? d - 2 * V * a.rot_units : d - rotated;
-  a.units = a.rot_units + (in_place || rest <= 0 ? 0 : (rest + 2 * V - 1) / (2 * V));
   const int sms = dh_sm_count();
   const int budget = (c.budget <= 0 || c.budget > sms) ? sms : (int)c.budget;
   const cudaStream_t s = (cudaStream_t)c.stream;
-  // threads that share the heads of a row: enough of them to fill half of the GPU's threads, where there are that few rows
-  a.groups = 1;
-  while (a.groups * 2 <= heads_q + heads_k && rows * a.units * a.groups < (int64_t)budget * 1024) a.groups *= 2;
   // CTAs of a launch; beyond them they walk on.  On the whole GPU 8, 16, 32 per SM and as many as there are: 200000 x 40 heads of 128 661,
   // 637, 631 and 632 us, 500000 x 3 155, 153, 152 and 160 us.
   const int64_t cap = (int64_t)budget * (budget < sms ? 8 : 32);
+  // Through shared memory, where the pairs alone keep a vector at 4 bytes or fewer.  By the kernel above / so: 16384 x 80 heads of 96, 38
+  // rotated 212 / 92 us, 16384 x 40 of 128, 50 rotated 144 / 60, 16384 x 80 of 80, 20 rotated 109 / 76, fp32 16384 x 40 of 96, 38 rotated
+  // 110 / 88.  Not for small calls (30 x 40 heads of 96: 4.3 / 5.3 us, 100 x 40: 6.4 / 5.5), nor where 8 lanes' angles are for less than a
+  // step (65536 x 8 heads of 80, 20 rotated: 53 / 58 us; x 16: 91 / 85); at 8 bytes the kernel above has the fewer instructions.
+  const int all = heads_q + heads_k, words = !c.f32 && bytes == 4 ? a.half / 2 : a.half;
+  const int vecs = d * size / 16, per = vecs > 0 ? 32 * RS / vecs : 0;
+  if (bytes <= 4 && !interleaved && ((wide | (uint64_t)d * size) & 15) == 0 && per > 0 && a.half <= 128 && rows * all >= 4096 &&
+      (words > 8 || all >= per)) {
+    a.units = vecs;
+    a.groups = 1;
+    while (a.groups * 2 * per <= all && rows * a.groups < (int64_t)budget * 64) a.groups *= 2;
+    const int64_t most = INT32_MAX / a.groups;
+    for (int64_t r = 0; r < rows; r += most) {
+      a.row0 = r;
+      a.rows = rows - r < most ? rows - r : most;
+      const int64_t blocks = (a.rows * a.groups + RT / 32 - 1) / (RT / 32);
+      const int grid = (int)(blocks < cap ? blocks : cap);
+      if (c.f32) rope_launch_staged<float, 1>(a, words, grid, s);
+      else if (bytes == 4) rope_launch_staged<__nv_bfloat16, 2>(a, words, grid, s);
+      else rope_launch_staged<__nv_bfloat16, 1>(a, words, grid, s);
+    }
+    return rope_rc();
+  }
+  a.rot_units = (a.half + V - 1) / V;
+  const int rest = interleaved ? d - 2 * V * a.rot_units : d - rotated;
+  a.units = a.rot_units + (in_place || rest <= 0 ? 0 : (rest + 2 * V - 1) / (2 * V));
+  // threads that share the heads of a row: enough of them to fill half of the GPU's threads, where there are that few rows
+  a.groups = 1;
+  while (a.groups * 2 <= all && rows * a.units * a.groups < (int64_t)budget * 1024) a.groups *= 2;
   const int64_t most = INT32_MAX / ((int64_t)a.units * a.groups);      // rows of one launch: item numbers stay in 31 bits
   for (int64_t r = 0; r < rows; r += most) {
     a.row0 = r;
@@ -276,9 +428,7 @@ int dh_rope_heads(const void* call) {
       else rope_launch<__nv_bfloat16, 1>(a, interleaved, grid, s);
     }
   }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) set_last_error_c("dh_rope_heads", cudaGetErrorString(e));
-  return (int)e;
+  return rope_rc();
 }
 
 }  // extern "C"

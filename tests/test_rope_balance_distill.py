@@ -326,6 +326,6 @@ def test_sizes_beyond_31_bits_of_a_loop_are_refused():
         c = M._ROUTER_CALL.pack(0, E, 0, k, 0, 0, T, E, k, 0, 0)
         assert call("dh_balance_fwd", M._BALANCE_FWD, c, 0, 0, 0, 0) != 0
         assert call("dh_router_bwd", M._ROUTER_BWD, c, 0, k, 0, k, 0, 0.0, 0) != 0
-    for heads_q, heads_k in (((1 << 29) + 1, 1), (0, (1 << 29) + 1)):
+    for heads_q, heads_k in (((1 << 28) + 1, 1), (0, (1 << 28) + 1)):
         c = R._ROPE_CALL.pack(*[0] * 16, heads_q, heads_k, 0, 0, 0, 1, 1, 2, 2, 0, 0, 0, 0, 0, 1.0)
         assert call("dh_rope_heads", R._ROPE_ARGS, c) != 0

@@ -75,6 +75,41 @@ def test_rope_strides_alignment_and_far_positions(dtype, interleaved):
     check_rope(four, None, pos, freq, interleaved, 0.9, sm_budget=3)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("T,H,Hk,d,r", [(700, 5, 1, 96, 38), (1500, 2, 1, 128, 50), (310, 12, 3, 256, 102), (210, 17, 4, 80, 20), (900, 4, 1, 128, 100),
+                                        (700, 5, 2, 192, 76), (300, 15, 7, 64, 14), (1500, 2, 1, 256, 254), (4100, 1, 0, 96, 2), (4099, 1, 1, 96, 62),
+                                        (260, 100, 3, 16, 6), (2100, 1, 1, 512, 250), (9000, 1, 0, 8, 6)])
+def test_rope_halves_of_odd_numbers_of_pairs(T, H, Hk, d, r, dtype):
+    """Heads that pass through shared memory: odd halves and halves of 4k + 2, one to four rounds of a warp's lanes, heads that leave a step
+    unfilled, queries alone; contiguous, as views of a packed projection, in place, sequence-first, on few SMs."""
+    torch.manual_seed(T + r)
+    freq, scale = R.rope_frequencies(r, 500000.0, R.RopeScaling("llama3", 8.0), DEV)
+    pos = torch.randint(0, 1 << 20, (T,), device=DEV)
+    buf = torch.randn(T, H + 2 * Hk + 1, d, device=DEV).to(dtype)
+    q, k = buf[:, :H], buf[:, H:H + Hk] if Hk else None
+    check_rope(q, k, pos, freq, False, scale)
+    check_rope(q.contiguous(), None if k is None else k.contiguous(), pos, freq, False, scale, sm_budget=2)
+    want, keep = R.rope_fwd(q, k, pos, freq, scale=scale), buf.clone()
+    few = R.rope_fwd(q[5:9], None, pos[5:9], freq, scale=scale)[0]          # a few rows take the other kernel: the same bits
+    assert torch.equal(few, want[0][5:9])
+    R.rope_fwd(q, k, pos, freq, scale=scale, out=(q, k))
+    assert torch.equal(q, want[0]) and (k is None or torch.equal(k, want[1]))
+    assert torch.equal(buf[:, H + Hk:], keep[:, H + Hk:]) and torch.equal(buf[:, :H + Hk, r:], keep[:, :H + Hk, r:])
+    if T % 10 == 0:
+        four = keep.view(10, T // 10, H + 2 * Hk + 1, d).transpose(0, 1)
+        got = R.rope_fwd(four[:, :, :H], None, pos.view(10, -1).t().contiguous(), freq, scale=scale)[0]
+        assert torch.equal(got.transpose(0, 1).reshape(T, H, d), want[0])
+
+
+def test_rope_copies_what_it_does_not_turn_bit_by_bit():
+    g = torch.Generator().manual_seed(8)
+    bits = torch.randint(-32768, 32768, (900, 6, 96), generator=g, dtype=torch.int16).to(DEV)
+    x, pos = bits.view(BF), torch.arange(900, device=DEV)
+    for r, interleaved in ((38, False), (38, True), (32, False), (20, False), (22, True)):
+        q, k = R.rope_fwd(x[:, :5], x[:, 5:], pos, R.rope_frequencies(r, 10000.0, device=DEV)[0], interleaved=interleaved)
+        assert torch.equal(torch.cat([q, k], 1).view(torch.int16)[..., r:], bits[..., r:])
+
+
 def test_rope_in_place_leaves_the_rest_of_the_buffer():
     torch.manual_seed(4)
     buf = torch.randn(50, 10, 64, device=DEV).to(BF)
