@@ -34,7 +34,7 @@
 namespace dh {
 
 constexpr int D_MAX_K = 1024;
-constexpr int D_TABLE = 4096;            // slots for the entries of a row in the backward
+constexpr int D_AHEAD = 2;               // entries of a thread that the forward asks for at a time
 constexpr int D_BATCH = 4;               // 16-byte loads of a thread at a time
 constexpr float D_LOG2E = 1.4426950408889634f;
 constexpr float D_LN2 = 0.6931471805599453f;
@@ -193,6 +193,17 @@ __device__ __forceinline__ int d_id(const DistillArgs& a, int64_t row, int j) {
   const int64_t i = row * a.id_stride + j;
   const int64_t v = a.id64 ? reinterpret_cast<const int64_t*>(a.ids)[i] : (int64_t)reinterpret_cast<const int*>(a.ids)[i];
   return v < 0 || v >= a.V ? -1 : (int)v;
+}
+
+// Entries j, j + DT, ... of a row: ids (-1: padding or none) and logits.
+template <int DT, int N>
+__device__ __forceinline__ void d_entries(const DistillArgs& a, int64_t row, int j, int (&id)[N], float (&t)[N]) {
+#pragma unroll
+  for (int u = 0; u < N; ++u) {
+    id[u] = -1;
+    t[u] = 0.f;
+    if (j + u * DT < a.K) { id[u] = d_id(a, row, j + u * DT); t[u] = d_teacher(a, row, j + u * DT); }
+  }
 }
 
 // A row's elements in 16-byte vectors of the memory they lie in: `lead` elements before the first, then `vecs`, the rest behind them.
@@ -366,8 +377,14 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     float tm = -INFINITY;
     if (id0 >= 0) tm = t0;
     if (part == 0)
-      for (int j = threadIdx.x + DT; j < a.K; j += DT)
-        if (d_id(a, row, j) >= 0) tm = d_max(tm, d_teacher(a, row, j));
+      for (int j = threadIdx.x + DT; j < a.K; j += D_AHEAD * DT) {
+        int id[D_AHEAD];
+        float t[D_AHEAD];
+        d_entries<DT>(a, row, j, id, t);
+#pragma unroll
+        for (int u = 0; u < D_AHEAD; ++u)
+          if (id[u] >= 0) tm = d_max(tm, t[u]);
+      }
     float m, top;
     auto round = [&]() {
       const float wm = d_warp_max(acc.m), wt = d_warp_max(tm);
@@ -389,22 +406,29 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     tm = top;
     // second round: the sums; the teacher's relative to its largest
     float v[6] = {s1 * d_ex2((acc.m - m) * c1), st * d_ex2((acc.m - m) * ct), 0.f, 0.f, 0.f, 0.f};
-    if (part == 0 && tm != -INFINITY)
-      for (int j = threadIdx.x; j < a.K; j += DT) {
-        const bool early = j == (int)threadIdx.x;
-        const int id = early ? id0 : d_id(a, row, j);
-        if (id < 0) continue;
-        const float lt = ((early ? t0 : d_teacher(a, row, j)) - tm) * a.inv_tau;
-        const float q = expf(lt);
-        if (q == 0.f) continue;                          // no weight: its logit may be infinite
+    if (part == 0 && tm != -INFINITY) {
+      auto entry = [&](int id, float t, float zj) {
+        if (id < 0) return;
+        const float lt = (t - tm) * a.inv_tau, q = expf(lt);
+        if (q == 0.f) return;                            // no weight: its logit may be infinite
         v[2] += q;
         v[3] += q * lt;
-        const int loc = id - a.v0;
-        if (loc >= 0 && loc < a.Vl) {
-          v[4] += q * (((early ? z0 : d_load(z + loc)) - m) * ct);
+        if (id - a.v0 >= 0 && id - a.v0 < a.Vl) {
+          v[4] += q * ((zj - m) * ct);
           v[5] += q;
         }
+      };
+      entry(id0, t0, z0);
+      for (int j = threadIdx.x + DT; j < a.K; j += D_AHEAD * DT) {
+        int id[D_AHEAD];
+        float t[D_AHEAD], zj[D_AHEAD];
+        d_entries<DT>(a, row, j, id, t);
+#pragma unroll
+        for (int u = 0; u < D_AHEAD; ++u) zj[u] = id[u] - a.v0 >= 0 && id[u] - a.v0 < a.Vl ? d_load(z + (id[u] - a.v0)) : 0.f;
+#pragma unroll
+        for (int u = 0; u < D_AHEAD; ++u) entry(id[u], t[u], zj[u]);
       }
+    }
 #pragma unroll
     for (int q = 0; q < 6; ++q) v[q] = d_warp_sum(v[q]);
     if (lane == 0) {
@@ -487,15 +511,15 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
                                                             int64_t out_ld, int slots) {
   constexpr int N = DVec<T>::N;
   // Entries of this part that get more than the softmax: the teacher's, then the label.  An id may stand twice (often the label among the
-  // teacher's), so the first entry of an id writes for all: `first` has the lowest entry of each hash slot, which settles nearly all
-  // of them; only entries that met another id there, and first entries with twins, look through the list (K^2 steps without it:
-  // 256 entries took 113 of 457 us at 4096 x 128256).
+  // teacher's), so one entry of an id writes for all: the one that gets the id's place in a table, half of which stays empty.  Only
+  // entries with twins look through the list, and add up in its order (K^2 steps without the table: 256 entries took 113 of 457 us at
+  // 4096 x 128256).
   extern __shared__ __align__(16) int d_shared[];
-  int* first = d_shared;                    // [slots]
-  int* ids = first + slots;                 // [K + 1], -1: not in this part
+  int* table = d_shared;                    // [slots] entries, -1: empty
+  int* ids = table + slots;                 // [K + 1], -1: not in this part
   float* add = reinterpret_cast<float*>(ids + a.K + 1);
   float* at = add + a.K + 1;
-  int* twins = reinterpret_cast<int*>(at + a.K + 1);
+  uint8_t* twins = reinterpret_cast<uint8_t*>(at + a.K + 1);      // 1: writes for others too, 2: another one writes
   const int part = blockIdx.x % parts;
   const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
   for (int back = blockIdx.x / parts; back < a.T; back += gridDim.x / parts) {
@@ -519,8 +543,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
       for (int b = 0; b < D_BATCH; ++b) u[b] = zv[i + b * DT];
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < slots / 4; j += DT) reinterpret_cast<int4*>(first)[j] = make_int4(INT_MAX, INT_MAX, INT_MAX, INT_MAX);
-    __syncthreads();
+    for (int j = threadIdx.x; j < slots / 4; j += DT) reinterpret_cast<int4*>(table)[j] = make_int4(-1, -1, -1, -1);
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       int loc = -1;
       float g = 0.f;
@@ -535,12 +558,20 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
       add[j] = g;
       at[j] = in ? d_load(z + loc) : 0.f;
       twins[j] = 0;
-      if (in) atomicMin(first + d_slot(loc, slots), j);
     }
     __syncthreads();
     for (int j = threadIdx.x; j <= a.K; j += DT) {
-      const int id = ids[j], f = id >= 0 ? first[d_slot(id, slots)] : j;
-      if (f != j && ids[f] == id) twins[f] = 1;
+      const int id = ids[j];
+      if (id < 0) continue;
+      for (int s = d_slot(id, slots);; s = (s + 1) & (slots - 1)) {        // ends: half of the slots stay empty
+        const int other = atomicCAS(table + s, -1, j);
+        if (other < 0) break;
+        if (ids[other] == id) {
+          twins[other] = 1;
+          twins[j] = 2;
+          break;
+        }
+      }
     }
     const F2 nm = f2(-sv.x, -sv.x), c1p = f2(c1, c1), ctp = f2(ct, ct), Ap = f2(A, A), Bp = f2(B, B);
     auto soft2 = [&](F2 v) {
@@ -585,19 +616,15 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
     for (int j = threadIdx.x; j <= a.K; j += DT) {
       const int id = ids[j];
       if (id < 0 || zero) continue;
-      const int f = first[d_slot(id, slots)];
-      if (f != j && ids[f] == id) continue;             // the first of its id writes for it
+      const int twin = twins[j];
+      if (twin == 2) continue;
       float g = add[j];
-      bool mine = true;
-      if (f != j || twins[j]) {
+      if (twin == 1) {
         g = 0.f;
-        for (int q = 0; q <= a.K; ++q) {
-          if (ids[q] != id) continue;
-          if (q < j) mine = false;
-          g += add[q];
-        }
+        for (int q = 0; q <= a.K; ++q)
+          if (ids[q] == id) g += add[q];
       }
-      if (mine) d_store(o + id, soft(at[j]) - g);
+      d_store(o + id, soft(at[j]) - g);
     }
   }
 }
@@ -648,10 +675,14 @@ static int d_mode(const DistillCall& c) {
 }
 // Threads of a CTA: four batches of loads each, as far as 32 to 256 threads give that.  A row has some microseconds of its own (the
 // entries, two rounds of reductions), so short rows take small CTAs and the SM holds more of them.  Forward / backward with 256, 64 and 32
-// threads at 16384 x 4000: 160 / 172, 66 / 76 and 54 / 68 us; with 128 and 64 at 16384 x 8000: 91 / 113 and 76 / 109 us.
+// threads at 16384 x 4000: 160 / 172, 66 / 76 and 54 / 68 us; with 128 and 64 at 16384 x 8000: 91 / 113 and 76 / 109 us.  Where there are
+// fewer rows than the GPU holds such CTAs, larger ones (2000 x 2000 forward: 23 us in clusters of two CTAs of 32, 8 with 64 threads).
 static int d_threads(const DistillCall& c, int per_vec) {
-  const int64_t vecs = c.Vl / per_vec;
-  return vecs >= 16 * 256 ? 256 : vecs >= 16 * 128 ? 128 : vecs >= 16 * 64 ? 64 : 32;
+  const int sms = dh_sm_count();
+  const int64_t vecs = c.Vl / per_vec, room = 1024ll * ((c.budget <= 0 || c.budget > sms) ? sms : c.budget);
+  int threads = vecs >= 16 * 256 ? 256 : vecs >= 16 * 128 ? 128 : vecs >= 16 * 64 ? 64 : 32;
+  while (threads < 256 && c.T * threads * 2 <= room && vecs >= threads) threads *= 2;
+  return threads;
 }
 // CTAs that share a row: where there are fewer rows than the GPU holds CTAs, as long as each thread still has a vector; `waves` > 1 (the
 // backward, whose parts need not be joined): up to that many times what the GPU holds while each thread has four batches, so that
@@ -707,8 +738,8 @@ static void d_launch_bwd_as(const DistillCall& c, const float4* saved, const flo
       distill_bwd_kernel<T, D_ONE, DT>, distill_bwd_kernel<T, D_TWO, DT>, distill_bwd_kernel<T, D_SQUARE, DT>, distill_bwd_kernel<T, D_FOURTH, DT>};
   const int parts = d_parts(c, DT, DVec<T>::N, 64, 8);
   int slots = 64;
-  while (slots < 8 * c.K && slots < D_TABLE) slots *= 2;
-  const size_t shared = sizeof(int) * (slots + 4 * (size_t)(c.K + 1));       // at most 32 KB
+  while (slots < 2 * (c.K + 1)) slots *= 2;
+  const size_t shared = sizeof(int) * (slots + 3 * (size_t)(c.K + 1)) + c.K + 1;       // at most 30 KB
   kernels[d_mode(c)]<<<d_grid(c, DT, parts), DT, shared, (cudaStream_t)c.stream>>>(d_args(c), parts, saved, g_ce, g_kd, out, out_ld, slots);
 }
 template <typename T>

@@ -472,6 +472,22 @@ def test_distill_all_entries_the_same_id():
         check_distill(case, tau, *run_distill(on_gpu(case), tau), F32)
 
 
+@pytest.mark.parametrize("T,V,K", [(3, 40, k) for k in (1, 31, 32, 33, 63, 127, 500, 1024)] + [(70, 3000, 31), (70, 3000, 127), (30, 3000, 1024),
+                                                                                                (1300, 700, 33), (200, 700, 500)])
+def test_distill_tables_of_entries(T, V, K):
+    """As many entries as a row's places, more entries than the vocabulary has ids (all of them twins), ids that fall on the same place of
+    the table, the label among them; few and many rows take CTAs of different sizes."""
+    case = z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, seed=K, scale=2.0)
+    ids[0] = torch.arange(K) % V                          # every id, in order
+    ids[T // 2] = (torch.arange(K) * 2048) % V            # and multiples of a power of two
+    labels[0], labels[T // 2] = 0, 2048 % V
+    there = on_gpu(case)
+    ce, kd, grad = run_distill(there, 1.7)
+    check_distill(case, 1.7, ce, kd, grad, F32)
+    for _ in range(3):
+        assert torch.equal(run_distill(there, 1.7)[2], grad)
+
+
 def test_distill_far_rows_of_a_long_batch():
     """Element offsets beyond 32 bits: the last rows of 2^31 + 2^23 logits."""
     T, V = 16450, 131072
