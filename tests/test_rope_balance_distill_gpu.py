@@ -213,6 +213,27 @@ def test_balance_many_tokens():
     assert bool(((got - want).abs() <= O.EPS32 * (E + 2 * k + 30) * size).all())
 
 
+@pytest.mark.parametrize("T,E,k,masked", [(30000, 61, 4, True), (20011, 90, 8, True), (20011, 134, 3, False), (9000, 135, 3, True), (3000, 1022, 2, True),
+                                          (3001, 1023, 2, False), (40000, 30, 2, True), (70001, 3, 2, True)])
+def test_balance_of_rows_that_are_no_vectors(T, E, k, masked):
+    """Experts that two or no fewer than one float divide, over several clusters and one; NaN where no token is counted; rows with a gap."""
+    probs, ids, gates, dg, mask = router_case(T, E, k, device=DEV, masked=masked)
+    wide = torch.full((T, E + E % 2 + 2), float("nan"), device=DEV)
+    wide[:, :E] = probs
+    if masked:
+        wide[~mask] = float("nan")
+    keep = torch.ones(T, dtype=torch.bool, device=DEV) if mask is None else mask
+    want, n = torch.bincount(ids[keep].reshape(-1), minlength=E), int(keep.sum())
+    coef = want.double() * E / (n * float(n) * k)
+    for p in (wide[:, :E], wide[:, :E].contiguous()):
+        loss, counts, bal = M.balance_loss_fwd(p, ids, mask)
+        assert torch.equal(counts.long(), want)
+        # chains of a thread's rows, of the threads and clusters that hold an expert, and of the experts
+        assert math.isclose(float(loss), float((coef * probs[keep].double().sum(0)).sum()), rel_tol=O.EPS32 * (400 + T / 64))
+        assert bool(((bal.coef.double() - coef).abs() <= 8 * O.EPS32 * coef).all())
+        assert torch.equal(M.balance_loss_fwd(p, ids, mask)[0], loss)
+
+
 def test_balance_strides_empty_masks_and_masked_values():
     T, E, k = 200, 12, 3
     probs, ids, gates, dg, mask = router_case(T, E, k, device=DEV)
