@@ -383,12 +383,14 @@ static int bal_budget(const BalCall& c) {
   return (c.budget <= 0 || c.budget > sms) ? sms : (int)c.budget;
 }
 static bool bal_aligned(const BalCall& c, int w) { return c.E % w == 0 && c.p_stride % w == 0 && c.probs % (4 * w) == 0; }
-// Clusters of the forward: one (a single launch) up to B_ALONE probabilities, beyond it two CTAs of 256 threads per SM (65536 x 256: 21 us,
-// with four of them 25, with one of 1024 threads 34).  A budget of fewer SMs than a cluster's CTAs still takes one cluster.
+// Clusters of the forward: one (a single launch) up to B_ALONE probabilities and choices (65536 x 8 with 8 choices alone 21 us, in several
+// 12; 5003 x 61 12 us either way, with a launch and an allocation fewer), beyond it two CTAs of 256 threads per SM (65536 x 256: 21 us, with four of them 25, with one of
+// 1024 threads 34).  A budget of fewer SMs than a cluster's CTAs still takes one cluster.
 constexpr int64_t B_ALONE = 1 << 19;
 static int bal_clusters(const BalCall& c) {
-  if (c.T * c.E <= B_ALONE) return 1;
-  const int64_t want = c.T * c.E / (1 << 14) / B_CLUSTER, most = 2 * bal_budget(c) / B_CLUSTER;
+  const int64_t work = c.T * (c.E + c.k);
+  if (work <= B_ALONE) return 1;
+  const int64_t want = work / (1 << 14) / B_CLUSTER, most = 2 * bal_budget(c) / B_CLUSTER;
   const int64_t n = want < most ? want : most;
   return n < 1 ? 1 : (int)n;
 }
