@@ -13,7 +13,7 @@
 // below what its own rounding loses.  Exponentials are 2^(z c - R) in one fma, with c = log2 e or log2 e / tau and R = m c rounded; the
 // rounding of R is taken out of the sum when the thread is done.  A row whose maximum is
 // beyond D_FAR powers of two (the type's lowest value everywhere) has a slow form, the difference first.  The teacher's sums are linear in
-// exp(t / tau), so one CTA needs two rounds of reductions in all.  Sums are fp32.
+// exp(t / tau), so a row needs two rounds of reductions in all; CTAs that share a row join their maxima in the first.  Sums are fp32.
 // Backward: one pass computes every element from (m, 1 / sum, 1 / sum at tau) and the few entries with a label or a teacher's weight are
 // written once more behind it, from logits read before it, so that each element is rounded once.
 //
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
   extern __shared__ __align__(16) uint4 d_ring[];          // [2][D_BATCH][DT]: a thread's vectors pass through its own slots
   __shared__ float red[2][DW];
   __shared__ float sums[DW][6];
-  __shared__ float join[4];                          // this CTA's m, s1, st for the first one of its cluster
+  __shared__ float join[4];                          // for the cluster: this CTA's maximum (fast and slow form), s1, st
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int part = blockIdx.x % parts;
   const float ct = D_LOG2E * a.inv_tau, c1 = D_LOG2E;
@@ -373,7 +373,9 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     const int tail = sp.lead + sp.vecs * N + (int)threadIdx.x;
     if (part == 0 && (int)threadIdx.x < sp.lead) single(threadIdx.x);
     if (part == parts - 1 && tail < a.Vl) single(tail);
-    // first round: the CTA's reference and the teacher's largest logit
+    // first round: the row's reference, which all CTAs that share the row take before they form anything relative to it (their own
+    // shares may lie far below: a masked part of the vocabulary; the exchange takes 0.3 to 0.8 us, 17 x 128256: 7.3 -> 7.8 us), and the
+    // teacher's largest logit
     float tm = -INFINITY;
     if (id0 >= 0) tm = t0;
     if (part == 0)
@@ -386,7 +388,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
           if (id[u] >= 0) tm = d_max(tm, t[u]);
       }
     float m, top;
-    auto round = [&]() {
+    auto round = [&](int slot) {
       const float wm = d_warp_max(acc.m), wt = d_warp_max(tm);
       if (lane == 0) { red[0][w] = wm; red[1][w] = wt; }
       __syncthreads();
@@ -394,14 +396,20 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
       top = red[1][0];
 #pragma unroll
       for (int q = 1; q < DW; ++q) { m = d_max(m, red[0][q]); top = d_max(top, red[1][q]); }
+      if (parts > 1) {
+        if (threadIdx.x == 0) join[slot] = m;
+        __syncwarp();
+        cluster_sync_all();
+        m = d_warp_max(lane < parts ? __uint_as_float(ld_cluster_u32(mapa_u32(smem_u32(join + slot), lane))) : -INFINITY);
+      }
     };
-    round();
+    round(0);
     if (!(m > -far && m < far)) {
       acc.m = -FLT_MAX;
       s1 = st = 0.f;
       for (int c = sp.c0 + threadIdx.x; c < sp.c1; c += DT) single(c);
       __syncthreads();
-      round();
+      round(1);
     }
     tm = top;
     // second round: the sums; the teacher's relative to its largest
@@ -444,23 +452,17 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
       }
 #pragma unroll
       for (int q = 0; q < 6; ++q) v[q] = __shfl_sync(0xffffffffu, t, q);
-      if (lane == 0 && parts > 1) { join[0] = m; join[1] = v[0]; join[2] = v[1]; }
+      if (lane == 0 && parts > 1) { join[2] = v[0]; join[3] = v[1]; }
     }
     __syncwarp();
     if (parts > 1) cluster_sync_all();
     if (part == 0 && threadIdx.x == 0) {
       float dot = v[4], own = v[5];
-      float target = lin ? (zl - m) * c1 : INFINITY;
+      const float target = lin ? (zl - m) * c1 : INFINITY;
       for (int r = 1; r < parts; ++r) {
         const uint32_t at = mapa_u32(smem_u32(join), r);
-        const float om = __uint_as_float(ld_cluster_u32(at)), o1 = __uint_as_float(ld_cluster_u32(at + 4)),
-                    ot = __uint_as_float(ld_cluster_u32(at + 8));
-        const float to = d_max(m, om);
-        v[0] = v[0] * d_ex2((m - to) * c1) + o1 * d_ex2((om - to) * c1);
-        v[1] = v[1] * d_ex2((m - to) * ct) + ot * d_ex2((om - to) * ct);
-        if (own != 0.f) dot += own * ((m - to) * ct);
-        target += (m - to) * c1;
-        m = to;
+        v[0] += __uint_as_float(ld_cluster_u32(at + 8));
+        v[1] += __uint_as_float(ld_cluster_u32(at + 12));
       }
       if (MODE == D_ONE) v[0] = v[1];
       const float ent = tm != -INFINITY ? v[3] / v[2] - logf(v[2]) : INFINITY;

@@ -526,3 +526,54 @@ def test_distill_gpu_refusals():
     for bad in (dict(logits=z.half()), dict(logits=z.t().contiguous().t()), dict(labels=labels.cpu()), dict(top_ids=ids.cpu())):
         with pytest.raises(ValueError):
             L.vocab_parallel_distill_fwd(**(dict(logits=z, labels=labels, top_ids=ids, top_logits=top) | bad))
+
+
+def masked_parts(T, V, K, dtype, low, live, seed):
+    """``(case, exact)``: rows of which only the columns ``live`` are not ``low``; labels and entries lie there, rows 1, 5, ... have no label.
+    ``exact`` has -inf in place of ``low``: from -1e4 on both weigh nothing, in 64 bits either (temperatures up to 4)."""
+    a, b = live
+    z, labels, ids, top, g_ce, g_kd = distill_case(T, b - a, K, seed=seed, dtype=dtype)
+    labels, ids = torch.where((labels >= 0) & (labels < b - a), labels + a, -100), torch.where((ids >= 0) & (ids < b - a), ids + a, -1)
+    labels[1::4] = -100
+    case, exact = (torch.full((T, V), v, dtype=dtype) for v in (low, float("-inf")))
+    case[:, a:b] = exact[:, a:b] = z
+    rest = (labels, ids.to(torch.int32), top, g_ce, g_kd)
+    return (case, *rest), (exact, *rest)
+
+
+@pytest.mark.parametrize("low", [-1e4, -1e6, -1e9, "lowest", float("-inf")])
+@pytest.mark.parametrize("T,V,dtype", [(3, 3000, F32), (200, 5000, F32), (1, 40000, BF), (3, 40001, F32), (17, 128256, BF)])
+def test_distill_masked_parts_of_shared_rows(T, V, dtype, low):
+    """Rows that 2 to 8 CTAs share, of which the first eighth, the first half, or all but the last eighth, is masked: the shares of the
+    label and of the teacher's entries are far above other shares; no label is no label whatever is masked."""
+    low = torch.finfo(dtype).min if low == "lowest" else low
+    for part, live in enumerate(((V // 8, V), (V // 2, V), (V - V // 8, V), (V // 3, V // 2))):
+        case, exact = masked_parts(T, V, 9, dtype, low, live, seed=V + part)
+        for tau in (1.0, 1.5, 2.0, 4.0):
+            ce, kd, grad = run_distill(on_gpu(case), tau)
+            check_distill(exact, tau, ce, kd, grad, dtype)
+            assert float(ce[1::4].abs().sum()) == 0.0
+
+
+@pytest.mark.parametrize("low", [-1e9, "lowest", float("-inf")])
+def test_distill_masked_parts_of_shared_rows_are_what_many_rows_give(low):
+    """The same rows held by one CTA each, in a call of many, and as two shards of which one is masked as a whole."""
+    low = torch.finfo(F32).min if low == "lowest" else low
+    case, exact = masked_parts(4, 6000, 7, F32, low, (3000, 6000), seed=6)
+    many = tuple(t.repeat(*([400] + [1] * (t.dim() - 1))) for t in case)
+    few, all_rows = run_distill(on_gpu(case), 1.7), run_distill(on_gpu(many), 1.7)
+    check_distill(exact, 1.7, *few, F32)
+    check_distill(exact, 1.7, *(t[800:804] for t in all_rows), F32)
+    z, labels, ids, top, g_ce, g_kd = on_gpu(case)
+    stats = []
+    with pytest.MonkeyPatch.context() as patch:
+        patch.setattr(L, "group_size", lambda group: 2)
+        patch.setattr(L.dist, "all_gather_into_tensor", lambda every, mine, group=None: stats.append(mine.clone()))
+        for v0 in (0, 3000):
+            L.vocab_parallel_distill_fwd(z[:, v0:v0 + 3000], labels, ids, top, 1.7, vocab_start=v0)
+        patch.setattr(L.dist, "all_gather_into_tensor", lambda every, mine, group=None: every.copy_(torch.cat(stats)))
+        ce, kd, saved = L.vocab_parallel_distill_fwd(z[:, :3000], labels, ids, top, 1.7)
+    grad = torch.empty_like(z)
+    for v0 in (0, 3000):
+        L.vocab_parallel_distill_bwd_(z[:, v0:v0 + 3000], labels, ids, top, saved, g_ce, g_kd, 1.7, vocab_start=v0, out=grad[:, v0:v0 + 3000])
+    check_distill(exact, 1.7, ce, kd, grad, F32)
