@@ -264,13 +264,14 @@ struct DSums {
   }
 };
 
-// What a row's sums give.  m: reference; s1, st: sums; target: (z_label - m) log2 e (+inf: no label here); dot, own: sums of q (z_id - m)
-// log2 e / tau and of q over the entries here; ent: sum of q log q (+inf: the row has no entries); tl: the teacher's lse at tau.
+// What a row's sums give.  m: reference; s1, st: sums; target: z_label - m (+inf: no label here); dot, own: sums of q (z_id - m) and of q
+// over the entries here; ent: sum of q log q (+inf: the row has no entries); tl: the teacher's lse at tau.  Differences of logits carry no
+// factor: they may be as large as the type's lowest value.
 __device__ __forceinline__ void d_finish(float m, float s1, float st, float target, float dot, float ent, float tl, float tau, float* ce,
                                          float* kd, float4* saved) {
   const bool hard = target != INFINITY && s1 != 0.f, soft = ent != INFINITY && st != 0.f;      // a sum of 0: all logits are -inf
-  if (ce != nullptr) *ce = hard ? D_LN2 * (log2f(s1) - target) : 0.f;
-  *kd = soft ? tau * tau * (ent + D_LN2 * (log2f(st) - dot)) : 0.f;
+  if (ce != nullptr) *ce = hard ? D_LN2 * log2f(s1) - target : 0.f;
+  *kd = soft ? tau * (tau * (ent + D_LN2 * log2f(st)) - dot) : 0.f;
   *saved = make_float4(m, hard ? 1.f / s1 : 0.f, soft ? 1.f / st : 0.f, soft ? tl : INFINITY);
 }
 
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
         v[2] += q;
         v[3] += q * lt;
         if (id - a.v0 >= 0 && id - a.v0 < a.Vl) {
-          v[4] += q * ((zj - m) * ct);
+          v[4] += q * ((zj - m) * (1.f / D_MAX_K));        // a power of two: the sum of all entries stays finite
           v[5] += q;
         }
       };
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
     if (parts > 1) cluster_sync_all();
     if (part == 0 && threadIdx.x == 0) {
       float dot = v[4], own = v[5];
-      const float target = lin ? (zl - m) * c1 : INFINITY;
+      const float target = lin ? zl - m : INFINITY;
       for (int r = 1; r < parts; ++r) {
         const uint32_t at = mapa_u32(smem_u32(join), r);
         v[0] += __uint_as_float(ld_cluster_u32(at + 8));
@@ -467,7 +468,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
       if (MODE == D_ONE) v[0] = v[1];
       const float ent = tm != -INFINITY ? v[3] / v[2] - logf(v[2]) : INFINITY;
       const float tl = tm != -INFINITY ? tm * a.inv_tau + logf(v[2]) : INFINITY;
-      if (own != 0.f) { dot /= v[2]; own /= v[2]; }
+      if (own != 0.f) { dot = dot / v[2] * D_MAX_K; own /= v[2]; }
       if (stats != nullptr) {
         stats[(size_t)row * 2] = make_float4(m, v[0], v[1], target);
         stats[(size_t)row * 2 + 1] = make_float4(dot, own, ent, tl);
@@ -495,8 +496,8 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const float4* __re
     const float d = u.x - m;
     s1 += u.y * d_ex2(d * D_LOG2E);
     st += u.z * d_ex2(d * ct);
-    if (u.w != INFINITY) target = u.w + d * D_LOG2E;
-    if (v.y != 0.f) dot += v.x + v.y * (d * ct);
+    if (u.w != INFINITY) target = u.w + d;
+    if (v.y != 0.f) dot += v.x + v.y * d;
     ent = v.z;
     tl = v.w;
   }

@@ -177,7 +177,7 @@ def _teacher_ref(top_ids, top_logits, vocab, temperature):
 
 
 def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature):
-    """``[T, 8]``: maximum m, sums of exp(z - m) and exp((z - m) / tau), z_label - m (+inf: the label is not here), sums of q (z_id - m) / tau
+    """``[T, 8]``: maximum m, sums of exp(z - m) and exp((z - m) / tau), z_label - m (+inf: the label is not here), sums of q (z_id - m)
     and q over the entries here, sum of q log q (+inf: the row has no entries), the teacher's log-sum-exp."""
     Vl = logits.shape[1]
     lf = logits.float()
@@ -187,7 +187,7 @@ def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, 
     loc = top_ids.long() - vocab_start
     own = (loc >= 0) & (loc < Vl) & (q != 0)
     zero, inf = torch.zeros_like(q), torch.full_like(m, float("inf"))
-    dot = torch.where(own, q * rel.gather(1, loc.clamp(0, Vl - 1)), zero).sum(1) / temperature
+    dot = torch.where(own, q * rel.gather(1, loc.clamp(0, Vl - 1)), zero).sum(1)
     ent = torch.where(q != 0, q * torch.log(torch.where(q != 0, q, 1.0)), zero).sum(1)
     target = inf
     if labels is not None:
@@ -206,10 +206,10 @@ def _distill_combine_ref(all_stats, temperature, hard):
     st = (all_stats[..., 2] * torch.exp(d / temperature)).sum(0)
     has, own, ent = all_stats[..., 3] != inf, all_stats[..., 5], all_stats[0, :, 6]
     target = torch.where(has, all_stats[..., 3] + d, 0.0).sum(0)
-    dot = torch.where(own != 0, all_stats[..., 4] + own * (d / temperature), 0.0).sum(0)
+    dot = torch.where(own != 0, all_stats[..., 4] + own * d, 0.0).sum(0)
     is_hard, is_soft = has.any(0) & (s1 != 0), (ent != inf) & (st != 0)       # a sum of 0: all logits of the row are -inf
     ce = torch.where(is_hard, torch.log(s1) - target, 0.0) if hard else None
-    kd = torch.where(is_soft, temperature ** 2 * (ent - dot + torch.log(st)), 0.0)
+    kd = torch.where(is_soft, temperature * (temperature * (ent + torch.log(st)) - dot), 0.0)
     return ce, kd, torch.stack([m, torch.where(is_hard, 1.0 / s1, 0.0), torch.where(is_soft, 1.0 / st, 0.0),
                                 torch.where(is_soft, all_stats[0, :, 7], inf)], dim=1)
 

@@ -329,3 +329,34 @@ def test_sizes_beyond_31_bits_of_a_loop_are_refused():
     for heads_q, heads_k in (((1 << 28) + 1, 1), (0, (1 << 28) + 1)):
         c = R._ROPE_CALL.pack(*[0] * 16, heads_q, heads_k, 0, 0, 0, 1, 1, 2, 2, 0, 0, 0, 0, 0, 1.0)
         assert call("dh_rope_heads", R._ROPE_ARGS, c) != 0
+
+
+def lowest_case(T, V, K, dtype, seed):
+    """Rows whose label or whose teacher's entries, one of them up to most, lie on logits of the type's lowest value: losses near the end of
+    what fp32 holds."""
+    z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, seed=seed, dtype=dtype, scale=1.0)
+    g = torch.Generator().manual_seed(seed)
+    ids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(T)]).to(torch.int32)
+    labels = torch.randint(0, V, (T,), generator=g, dtype=torch.int32)
+    low = torch.finfo(dtype).min
+    for t in range(T):
+        if t % 3 == 0:
+            z[t, labels[t]] = low
+        if t % 3 == 1:
+            z[t, ids[t, -1]] = low
+            top[t, -1] = top[t].max() - 2.0
+        if t % 3 == 2:
+            z[t, ids[t, : K // 5].long()] = low
+            top[t] = 4.0
+    return z, labels, ids, top, g_ce, g_kd
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.7, 3.3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_distill_losses_near_the_end_of_the_type(dtype, tau):
+    """A weight of at most 1/5 on 3.4e38 at a temperature of at most 3.3: the exact losses are fp32 numbers."""
+    case = z, labels, ids, top, g_ce, g_kd = lowest_case(9, 400, 50, dtype, 3)
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
+    grad = L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, tau)
+    assert bool(torch.isfinite(ce).all()) and bool(torch.isfinite(kd).all())
+    check_distill(case, tau, ce, kd, grad, dtype)

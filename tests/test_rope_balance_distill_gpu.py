@@ -9,7 +9,7 @@ import operator_oracles as O
 from dhellam_b200.ops import loss as L
 from dhellam_b200.ops import moe as M
 from dhellam_b200.ops import rope as R
-from test_rope_balance_distill import check_distill, distill_case, router_case
+from test_rope_balance_distill import check_distill, distill_case, lowest_case, router_case
 
 pytestmark = pytest.mark.gpu
 
@@ -577,3 +577,12 @@ def test_distill_masked_parts_of_shared_rows_are_what_many_rows_give(low):
     for v0 in (0, 3000):
         L.vocab_parallel_distill_bwd_(z[:, v0:v0 + 3000], labels, ids, top, saved, g_ce, g_kd, 1.7, vocab_start=v0, out=grad[:, v0:v0 + 3000])
     check_distill(exact, 1.7, ce, kd, grad, F32)
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.7, 3.3])
+@pytest.mark.parametrize("T,V,K,dtype", [(9, 400, 50, BF), (9, 400, 50, F32), (6, 40000, 1000, BF), (6, 20001, 700, F32), (700, 900, 40, BF)])
+def test_distill_losses_near_the_end_of_the_type(T, V, K, dtype, tau):
+    case = lowest_case(T, V, K, dtype, 3)
+    ce, kd, grad = run_distill(on_gpu(case), tau)
+    assert bool(torch.isfinite(ce).all()) and bool(torch.isfinite(kd).all())
+    check_distill(case, tau, ce, kd, grad, dtype)
