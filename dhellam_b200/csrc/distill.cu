@@ -14,7 +14,7 @@
 // rounding of R is taken out of the sum when the thread is done.  A row whose maximum is
 // beyond D_FAR powers of two (the type's lowest value everywhere) has a slow form, the difference first.  The teacher's sums are linear in
 // exp(t / tau), so a row needs two rounds of reductions in all; CTAs that share a row join their maxima in the first.  Sums are fp32.
-// Backward: one pass computes every element from (m, 1 / sum, 1 / sum at tau) and the few entries with a label or a teacher's weight are
+// Backward: one pass computes every element from m, 1 / sum and 1 / sum at tau, and the few entries with a label or a teacher's weight are
 // written once more behind it, from logits read before it, so that each element is rounded once.
 //
 // With both losses an element costs two exponentials, unless tau is 1 (they are the same) or 2 or 4 (exp(x) is a power of exp(x / tau):
@@ -265,20 +265,24 @@ struct DSums {
 };
 
 // What a row's sums give.  m: reference; s1, st: sums; target: z_label - m (+inf: no label here); dot, own: sums of q (z_id - m) and of q
-// over the entries here; ent: sum of q log q (+inf: the row has no entries); tl: the teacher's lse at tau.  Differences of logits carry no
-// factor: they may be as large as the type's lowest value.
-__device__ __forceinline__ void d_finish(float m, float s1, float st, float target, float dot, float ent, float tl, float tau, float* ce,
+// over the entries here; ent: sum of q log q (+inf: the row has no entries); tm, lv: the teacher's largest logit and log of its sum relative
+// to that.  Differences of logits carry no factor: they may be as large as the type's lowest value.
+// saved [4] pairs: (m, 0), (1 / s1 or 0 where ce has no gradient, 0), (1 / st, 0), (lv or +inf where kd has no gradient, tm).  tm / tau + lv
+// in one number would lose lv where a row's logits are far from zero.
+__device__ __forceinline__ void d_finish(float m, float s1, float st, float target, float dot, float ent, float lv, float tm, float tau, float* ce,
                                          float* kd, float4* saved) {
   const bool hard = target != INFINITY && s1 != 0.f, soft = ent != INFINITY && st != 0.f;      // a sum of 0: all logits are -inf
   if (ce != nullptr) *ce = hard ? D_LN2 * log2f(s1) - target : 0.f;
   *kd = soft ? tau * (tau * (ent + D_LN2 * log2f(st)) - dot) : 0.f;
-  *saved = make_float4(m, hard ? 1.f / s1 : 0.f, soft ? 1.f / st : 0.f, soft ? tl : INFINITY);
+  saved[0] = make_float4(m, 0.f, hard ? 1.f / s1 : 0.f, 0.f);
+  saved[1] = make_float4(soft ? 1.f / st : 0.f, 0.f, soft ? lv : INFINITY, tm);
 }
 
 // One cluster of CTAs per row (one CTA where there are rows enough); they share its vectors and the first one joins their sums.  CTAs
 // that stay and ask for the next row's logits while they reduce are slower (4096 x 128256: 182 us, 207 so): SMs are not equally far from
 // the memory, and whoever is done takes the next row.  Bound by memory: 180 us without the exponentials.
-// Where `stats` is given (the vocabulary is divided among ranks) a row's eight numbers go there: m, s1, st, target, dot, own, ent, tl.
+// Where `stats` is given (the vocabulary is divided among ranks) a row's numbers go there: m, s1, st, target, dot, own, ent, 0; and what is the
+// same on every rank, lv and tm, to `saved`.
 template <typename T, int MODE, int DT>
 __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const DistillArgs a, int parts, float* __restrict__ ce, float* __restrict__ kd,
                                                             float4* __restrict__ saved, float4* __restrict__ stats) {
@@ -466,14 +470,14 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
         v[1] += __uint_as_float(ld_cluster_u32(at + 12));
       }
       if (MODE == D_ONE) v[0] = v[1];
-      const float ent = tm != -INFINITY ? v[3] / v[2] - logf(v[2]) : INFINITY;
-      const float tl = tm != -INFINITY ? tm * a.inv_tau + logf(v[2]) : INFINITY;
+      const float lv = tm != -INFINITY ? logf(v[2]) : INFINITY, ent = tm != -INFINITY ? v[3] / v[2] - lv : INFINITY;
       if (own != 0.f) { dot = dot / v[2] * D_MAX_K; own /= v[2]; }
       if (stats != nullptr) {
         stats[(size_t)row * 2] = make_float4(m, v[0], v[1], target);
-        stats[(size_t)row * 2 + 1] = make_float4(dot, own, ent, tl);
+        stats[(size_t)row * 2 + 1] = make_float4(dot, own, ent, 0.f);
+        saved[(size_t)row * 2 + 1] = make_float4(0.f, 0.f, lv, tm);
       } else {
-        d_finish(m, v[0], v[1], target, dot, ent, tl, a.tau, ce != nullptr ? ce + row : nullptr, kd + row, saved + row);
+        d_finish(m, v[0], v[1], target, dot, ent, lv, tm, a.tau, ce != nullptr ? ce + row : nullptr, kd + row, saved + (size_t)row * 2);
       }
     }
     __syncwarp();
@@ -481,16 +485,15 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_fwd_kernel(const Distil
   }
 }
 
-// stats [R, T, 8] of the ranks -> ce [T] (nullable), kd [T], saved [T, 4] = (m, 1 / sum or 0 where ce has no gradient, 1 / sum at tau,
-// the teacher's lse at tau or +inf where kd has no gradient).
+// stats [R, T, 8] of the ranks, and lv and tm in saved -> ce [T] (nullable), kd [T], saved.
 __global__ void __launch_bounds__(256) distill_combine_kernel(const float4* __restrict__ stats, int R, int T, float tau, float* __restrict__ ce,
-                                                             float* __restrict__ kd, float4* __restrict__ saved) {
+                                                             float* __restrict__ kd, float4* saved) {
   const int t = blockIdx.x * 256 + threadIdx.x;
   if (t >= T) return;
   const float ct = D_LOG2E / tau;
   float m = stats[(size_t)t * 2].x;
   for (int r = 1; r < R; ++r) m = d_max(m, stats[((size_t)r * T + t) * 2].x);
-  float s1 = 0.f, st = 0.f, target = INFINITY, dot = 0.f, ent = 0.f, tl = 0.f;
+  float s1 = 0.f, st = 0.f, target = INFINITY, dot = 0.f, ent = 0.f;
   for (int r = 0; r < R; ++r) {
     const float4 u = stats[((size_t)r * T + t) * 2], v = stats[((size_t)r * T + t) * 2 + 1];
     const float d = u.x - m;
@@ -499,9 +502,9 @@ __global__ void __launch_bounds__(256) distill_combine_kernel(const float4* __re
     if (u.w != INFINITY) target = u.w + d;
     if (v.y != 0.f) dot += v.x + v.y * d;
     ent = v.z;
-    tl = v.w;
   }
-  d_finish(m, s1, st, target, dot, ent, tl, tau, ce != nullptr ? ce + t : nullptr, kd + t, saved + t);
+  const float4 teacher = saved[(size_t)t * 2 + 1];
+  d_finish(m, s1, st, target, dot, ent, teacher.z, teacher.w, tau, ce != nullptr ? ce + t : nullptr, kd + t, saved + (size_t)t * 2);
 }
 
 __device__ __forceinline__ int d_slot(int id, int slots) { return (int)(((unsigned int)id * 2654435761u) >> 16) & (slots - 1); }
@@ -530,9 +533,9 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
     const T* z = reinterpret_cast<const T*>(a.z) + row * a.ld;
     T* o = reinterpret_cast<T*>(out) + row * out_ld;
     const DSpan sp = d_span(z, a.Vl, part, parts);
-    const float4 sv = saved[row];
-    const float gc = a.labels != nullptr && sv.y != 0.f ? g_ce[row] : 0.f, gk = sv.w != INFINITY ? g_kd[row] * a.tau : 0.f;
-    const float A = gc != 0.f ? gc * sv.y : 0.f, B = gk != 0.f ? gk * sv.z : 0.f;
+    const float4 sv = saved[(size_t)row * 2], teacher = saved[(size_t)row * 2 + 1];
+    const float gc = a.labels != nullptr && sv.z != 0.f ? g_ce[row] : 0.f, gk = teacher.z != INFINITY ? g_kd[row] * a.tau : 0.f;
+    const float A = gc != 0.f ? gc * sv.z : 0.f, B = gk != 0.f ? gk * teacher.x : 0.f;
     const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(o)) & 15) == 0;
     const bool zero = gc == 0.f && gk == 0.f;        // a token without loss: zeros, whatever its logits
     const uint4* zv = reinterpret_cast<const uint4*>(z + sp.lead);
@@ -554,7 +557,7 @@ __global__ void __launch_bounds__(DT, 1024 / DT) distill_bwd_kernel(const Distil
         if (gc != 0.f) { loc = a.labels[row] - a.v0; g = gc; }
       } else if (gk != 0.f) {
         const int id = d_id(a, row, j);
-        if (id >= 0) { loc = id - a.v0; g = gk * expf(d_teacher(a, row, j) * a.inv_tau - sv.w); }
+        if (id >= 0) { loc = id - a.v0; g = gk * expf((d_teacher(a, row, j) - teacher.w) * a.inv_tau - teacher.z); }
       }
       const bool in = loc >= sp.c0 && loc < sp.c1;
       ids[j] = in ? loc : -1;
@@ -760,7 +763,8 @@ using namespace dh;
 
 extern "C" {
 
-// ce [T] (null without labels), kd [T], saved [T, 4] fp32; or, for a shard of a divided vocabulary, stats [T, 8] alone.
+// ce [T] (null without labels), kd [T], saved [T, 4] pairs of fp32; or, for a shard of a divided vocabulary, stats [T, 8] and the teacher's
+// part of saved.
 int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stats) {
   const DistillCall& c = *(const DistillCall*)call;
   if (int rc = d_refuse("dh_distill_fwd", c)) return rc;

@@ -166,24 +166,27 @@ def _distill_call(logits, labels, ids, top, vocab_start, vocab, temperature, sm_
 
 
 def _teacher_ref(top_ids, top_logits, vocab, temperature):
-    """``(q [T, K] fp32, log-sum-exp [T])``: the teacher's distribution over a row's entries (0 on padding) and its normaliser at the
-    temperature (+inf: the row has no entries)."""
-    t = torch.where((top_ids >= 0) & (top_ids < vocab), top_logits.float(), float("-inf")) / temperature
+    """``(q [T, K] fp32, tm [T], lv [T])``: the teacher's distribution over a row's entries (0 on padding), its largest logit and the log of
+    its sum relative to that (+inf: the row has no entries)."""
+    t = torch.where((top_ids >= 0) & (top_ids < vocab), top_logits.float(), float("-inf"))
     if not t.shape[1]:
-        return t, torch.full(t.shape[:1], float("inf"), device=t.device)
-    none = (t == float("-inf")).all(1)
-    lse = torch.where(none, float("inf"), torch.logsumexp(t, 1))
-    return torch.exp(t - lse[:, None]), lse
+        return t, t.new_zeros(t.shape[0]), t.new_full(t.shape[:1], float("inf"))
+    tm = t.max(1).values
+    none = tm == float("-inf")
+    tm = torch.where(none, 0.0, tm)
+    q = torch.exp((t - tm[:, None]) / temperature)
+    total = torch.where(none, float("inf"), q.sum(1))
+    return q / total[:, None], tm, torch.log(total)
 
 
 def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature):
-    """``[T, 8]``: maximum m, sums of exp(z - m) and exp((z - m) / tau), z_label - m (+inf: the label is not here), sums of q (z_id - m)
-    and q over the entries here, sum of q log q (+inf: the row has no entries), the teacher's log-sum-exp."""
+    """``stats [T, 8]`` and ``(tm, lv)`` of the teacher.  Stats: maximum m, sums of exp(z - m) and exp((z - m) / tau), z_label - m (+inf: the label is not here), sums of q (z_id - m)
+    and q over the entries here, sum of q log q (+inf: the row has no entries), 0."""
     Vl = logits.shape[1]
     lf = logits.float()
     m = lf.max(dim=-1).values.clamp_min(torch.finfo(torch.float32).min)
     rel = lf - m[:, None]
-    q, t_lse = _teacher_ref(top_ids, top_logits, vocab, temperature)
+    q, tm, lv = _teacher_ref(top_ids, top_logits, vocab, temperature)
     loc = top_ids.long() - vocab_start
     own = (loc >= 0) & (loc < Vl) & (q != 0)
     zero, inf = torch.zeros_like(q), torch.full_like(m, float("inf"))
@@ -195,10 +198,10 @@ def _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, 
         inside = (labels >= 0) & (labels < vocab) & (loc >= 0) & (loc < Vl)
         target = torch.where(inside, rel.gather(1, loc.clamp(0, Vl - 1)[:, None]).squeeze(1), inf)
     return torch.stack([m, torch.exp(rel).sum(1), torch.exp(rel / temperature).sum(1), target, dot, torch.where(own, q, zero).sum(1),
-                        torch.where(t_lse == inf, inf, ent), t_lse], dim=1)
+                        torch.where(lv == inf, inf, ent), torch.zeros_like(m)], dim=1), (tm, lv)
 
 
-def _distill_combine_ref(all_stats, temperature, hard):
+def _distill_combine_ref(all_stats, teacher, temperature, hard):
     m = all_stats[..., 0].max(dim=0).values
     inf = torch.full_like(m, float("inf"))
     d = all_stats[..., 0] - m
@@ -210,20 +213,22 @@ def _distill_combine_ref(all_stats, temperature, hard):
     is_hard, is_soft = has.any(0) & (s1 != 0), (ent != inf) & (st != 0)       # a sum of 0: all logits of the row are -inf
     ce = torch.where(is_hard, torch.log(s1) - target, 0.0) if hard else None
     kd = torch.where(is_soft, temperature * (temperature * (ent + torch.log(st)) - dot), 0.0)
-    return ce, kd, torch.stack([m, torch.where(is_hard, 1.0 / s1, 0.0), torch.where(is_soft, 1.0 / st, 0.0),
-                                torch.where(is_soft, all_stats[0, :, 7], inf)], dim=1)
+    tm, lv = teacher
+    saved = torch.stack([m, torch.where(is_hard, 1.0 / s1, 0.0), torch.where(is_soft, 1.0 / st, 0.0), torch.where(is_soft, lv, inf)], dim=1)
+    zero = torch.zeros_like(tm)
+    return ce, kd, torch.complex(saved, torch.stack([zero, zero, zero, tm], dim=1))
 
 
 def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature: float = 1.0, vocab_start: int = 0, group=None,
                                sm_budget: int = 0, stream=None):
-    """Cross entropy and distillation loss per token, ``(ce [T], kd [T], saved [T, 4])`` in fp32.
+    """Cross entropy and distillation loss per token, ``(ce [T], kd [T], saved [T, 4])``, losses in fp32.
 
     ``logits [T, V/t]`` are the student's (bf16 or fp32), this rank's shard of the vocabulary from ``vocab_start`` on.  ``top_ids [T, K]``
     and ``top_logits [T, K]`` are the ids and logits of the teacher's best entries, the same on every rank; an id outside the
     vocabulary is padding.  With ``q = softmax(top_logits / temperature)`` over a row's entries and the student's ``p = softmax(logits /
     temperature)`` over the whole vocabulary, ``kd = temperature^2 KL(q || p)``; rows without entries give 0.  ``ce`` is the cross entropy
     against ``labels [T]`` int32 (0 where the label lies outside the vocabulary), or ``None`` without labels.  A row whose logits are
-    all ``-inf`` has neither loss nor gradient.  ``saved`` goes to
+    all ``-inf`` has neither loss nor gradient.  ``saved`` (pairs of fp32 numbers, as complex64) goes to
     ``vocab_parallel_distill_bwd_``.  The ranks of ``group`` exchange eight numbers a token in one all-gather."""
     if stream is not None:
         return K.run_on_stream(stream, (logits, labels, top_ids, top_logits), lambda: vocab_parallel_distill_fwd(
@@ -242,20 +247,20 @@ def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature:
         fn = K.proto("dh_distill_fwd", _DISTILL_FWD)
         kd = logits.new_empty(T, dtype=torch.float32)
         ce = torch.empty_like(kd) if labels is not None else None
-        saved = logits.new_empty((T, 4), dtype=torch.float32)
+        saved = logits.new_empty((T, 4), dtype=torch.complex64)
         if ws == 1:
             K.check(fn(call, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), 0), what)
             return ce, kd, saved
         stats = logits.new_empty((T, 8), dtype=torch.float32)
-        K.check(fn(call, 0, 0, 0, stats.data_ptr()), what)
+        K.check(fn(call, 0, 0, saved.data_ptr(), stats.data_ptr()), what)
     else:
-        stats = _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature)
+        stats, teacher = _distill_stats_ref(logits, labels, top_ids, top_logits, vocab_start, vocab, temperature)
     every = stats
     if ws > 1:
         every = torch.empty((ws * T, 8), dtype=stats.dtype, device=stats.device)
         dist.all_gather_into_tensor(every, stats, group=group)
     if not native:
-        return _distill_combine_ref(every.view(ws, T, 8), temperature, labels is not None)
+        return _distill_combine_ref(every.view(ws, T, 8), teacher, temperature, labels is not None)
     fn = K.proto("dh_distill_combine", [c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_void_p, c_void_p])
     K.check(fn(every.data_ptr(), ws, T, temperature, K.ptr(ce), kd.data_ptr(), saved.data_ptr(), K.stream_ptr()), what)
     return ce, kd, saved
@@ -284,22 +289,22 @@ def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce
         raise ValueError(f"{what}: logits that are overwritten have room for every row")
     if (g_ce is None) != (labels is None):
         raise ValueError(f"{what}: labels and the gradient of their loss go together")
-    for t in (g_kd, g_ce, saved):
-        if t is not None and (t.dtype is not torch.float32 or t.shape != ((T, 4) if t is saved else (T,)) or not t.is_contiguous()):
-            raise ValueError(f"{what}: contiguous fp32 gradients [T] and saved statistics [T, 4], got {t.dtype} {tuple(t.shape)}")
+    for t, shape, dtype in ((g_kd, (T,), torch.float32), (g_ce, (T,), torch.float32), (saved, (T, 4), torch.complex64)):
+        if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
+            raise ValueError(f"{what}: contiguous fp32 gradients [T] and statistics [T, 4] as they were saved, got {t.dtype} {tuple(t.shape)}")
     if K.use_native(logits):
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out)
         call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature, sm_budget)
         fn = K.proto("dh_distill_bwd", _DISTILL_BWD)
         K.check(fn(call, saved.data_ptr(), K.ptr(g_ce), g_kd.data_ptr(), out.data_ptr(), out.stride(0)), what)
         return out
-    rel = logits.float() - saved[:, :1]
-    inv, inv_t, t_lse = saved[:, 1], saved[:, 2], saved[:, 3]
-    gk = torch.where(t_lse != float("inf"), g_kd, 0.0) * temperature
+    tm, (m, inv, inv_t, lv) = saved[:, 3].imag, saved.real.unbind(1)
+    rel = logits.float() - m[:, None]
+    gk = torch.where(lv != float("inf"), g_kd, 0.0) * temperature
     d = torch.where(gk[:, None] != 0, torch.exp(rel / temperature) * (gk * inv_t)[:, None], 0.0)
     loc = top_ids.long() - vocab_start
     own = (loc >= 0) & (loc < Vl) & (gk[:, None] != 0)
-    w = torch.where(own, torch.exp(top_logits.float() / temperature - t_lse[:, None]) * gk[:, None], 0.0)
+    w = torch.where(own, torch.exp((top_logits.float() - tm[:, None]) / temperature - lv[:, None]) * gk[:, None], 0.0)
     d.scatter_add_(1, loc.clamp(0, Vl - 1), -w)
     if labels is not None:
         loc = labels.long() - vocab_start

@@ -360,3 +360,32 @@ def test_distill_losses_near_the_end_of_the_type(dtype, tau):
     grad = L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, tau)
     assert bool(torch.isfinite(ce).all()) and bool(torch.isfinite(kd).all())
     check_distill(case, tau, ce, kd, grad, dtype)
+
+
+def far_teacher(T, V, K, dtype, teacher, low, seed):
+    """``(case, exact)``: teacher's logits that are all ``low`` (a row whose entries are masked: each has the same weight), or lie a power of two
+    above or below steps of a quarter; ``exact`` has them without that (a distribution does not change by it), so that its bounds are those
+    of small logits."""
+    z, labels, ids, top, g_ce, g_kd = distill_case(T, V, K, seed=seed, dtype=dtype)
+    g = torch.Generator().manual_seed(seed)
+    if low is None:
+        near = torch.randint(0, 8, (T, K), generator=g) / 4
+        far = near + (1 << 12) * (2 * torch.randint(0, 2, (T, 1), generator=g) - 1)
+    else:
+        near, far = torch.zeros(T, K), torch.full((T, K), float(low))
+    top = far.to(teacher)
+    assert bool((top.double() - top.double().amax(1, keepdim=True) == near.double() - near.double().amax(1, keepdim=True)).all())
+    return (z, labels, ids, top, g_ce, g_kd), (z, labels, ids, near, g_ce, g_kd)
+
+
+FAR_TEACHERS = [(torch.float32, None), (torch.float32, -1e9), (torch.bfloat16, -1e4), (torch.bfloat16, torch.finfo(torch.bfloat16).min),
+                (torch.float16, torch.finfo(torch.float16).min), (torch.float32, torch.finfo(torch.float32).min)]
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.5, 1.7])
+@pytest.mark.parametrize("teacher,low", FAR_TEACHERS)
+def test_distill_teachers_logits_far_from_zero(teacher, low, tau):
+    case, exact = far_teacher(12, 60, 16, torch.float32, teacher, low, 7)
+    z, labels, ids, top, g_ce, g_kd = case
+    ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
+    check_distill(exact, tau, ce, kd, L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, tau), torch.float32)

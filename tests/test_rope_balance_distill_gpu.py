@@ -9,7 +9,7 @@ import operator_oracles as O
 from dhellam_b200.ops import loss as L
 from dhellam_b200.ops import moe as M
 from dhellam_b200.ops import rope as R
-from test_rope_balance_distill import check_distill, distill_case, lowest_case, router_case
+from test_rope_balance_distill import FAR_TEACHERS, check_distill, distill_case, far_teacher, lowest_case, router_case
 
 pytestmark = pytest.mark.gpu
 
@@ -586,3 +586,26 @@ def test_distill_losses_near_the_end_of_the_type(T, V, K, dtype, tau):
     ce, kd, grad = run_distill(on_gpu(case), tau)
     assert bool(torch.isfinite(ce).all()) and bool(torch.isfinite(kd).all())
     check_distill(case, tau, ce, kd, grad, dtype)
+
+
+@pytest.mark.parametrize("tau", [1.0, 2.0, 0.5, 1.7])
+@pytest.mark.parametrize("teacher,low", FAR_TEACHERS)
+def test_distill_teachers_logits_far_from_zero(teacher, low, tau, monkeypatch):
+    """Rows that CTAs share, rows of one CTA, and two shards."""
+    for T, V, K in ((6, 30000, 16), (700, 300, 40), (9, 777, 700)):
+        case, exact = far_teacher(T, V, K, F32, teacher, low, 7)
+        check_distill(exact, tau, *run_distill(on_gpu(case), tau), F32)
+    case, exact = far_teacher(8, 4000, 16, F32, teacher, low, 8)
+    z, labels, ids, top, g_ce, g_kd = on_gpu(case)
+    sent = []
+    monkeypatch.setattr(L, "group_size", lambda group: 2)
+    monkeypatch.setattr(L.dist, "all_gather_into_tensor", lambda every, stats, group=None: sent.append(stats.clone()))
+    for v0 in (0, 2000):
+        L.vocab_parallel_distill_fwd(z[:, v0:v0 + 2000], labels, ids, top, tau, vocab_start=v0)
+    monkeypatch.setattr(L.dist, "all_gather_into_tensor", lambda every, stats, group=None: every.copy_(torch.cat(sent)))
+    grad = torch.empty_like(z)
+    for v0 in (0, 2000):                                                  # each rank has what its own call saved
+        part = z[:, v0:v0 + 2000]
+        ce, kd, saved = L.vocab_parallel_distill_fwd(part, labels, ids, top, tau, vocab_start=v0)
+        L.vocab_parallel_distill_bwd_(part, labels, ids, top, saved, g_ce, g_kd, tau, vocab_start=v0, out=grad[:, v0:v0 + 2000])
+    check_distill(exact, tau, ce, kd, grad, F32)
