@@ -645,9 +645,15 @@ struct DistillCall {
 static int d_refuse(const char* what, const DistillCall& c) {
   // 2^30: a row's or an element's number plus one step of a loop stays in 31 bits
   if (c.T >= 0 && c.T <= (1 << 30) && c.Vl > 0 && c.Vl <= (1 << 30) && c.K >= 0 && c.K <= D_MAX_K && c.v0 >= 0 && c.V >= c.v0 + c.Vl && c.V <= INT32_MAX &&
-      c.tau > 0. && 1. / c.tau <= FLT_MAX && (float)c.tau > 0.f && (float)c.tau <= FLT_MAX)
+      c.tau >= FLT_MIN && c.tau <= FLT_MAX)
     return 0;
-  set_last_error_c(what, "a shard inside a vocabulary of at most 2^31 - 1 entries, at most 2^30 rows and entries a shard, 1024 teacher's entries, a positive temperature");
+  set_last_error_c(what, "a shard inside a vocabulary of at most 2^31 - 1 entries, at most 2^30 rows and entries a shard, 1024 teacher's entries, a temperature that is a normal fp32 number");
+  return (int)cudaErrorInvalidValue;
+}
+// The statistics of a row are read and written as vectors.
+static int d_refuse_unaligned(const char* what, const void* a, const void* b) {
+  if ((((uintptr_t)a | (uintptr_t)b) & 15) == 0) return 0;
+  set_last_error_c(what, "statistics that start on 16 bytes");
   return (int)cudaErrorInvalidValue;
 }
 static int d_rc(const char* what, cudaError_t e) {
@@ -768,6 +774,7 @@ extern "C" {
 int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stats) {
   const DistillCall& c = *(const DistillCall*)call;
   if (int rc = d_refuse("dh_distill_fwd", c)) return rc;
+  if (int rc = d_refuse_unaligned("dh_distill_fwd", saved, stats)) return rc;
   if (c.T == 0) return 0;
   const cudaError_t e = c.f32 ? d_launch_fwd<float>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats)
                               : d_launch_fwd<__nv_bfloat16>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats);
@@ -775,12 +782,14 @@ int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stat
 }
 int dh_distill_combine(const void* stats, int R, int T, float tau, void* ce, void* kd, void* saved, cudaStream_t s) {
   if (R <= 0 || T <= 0) return 0;
+  if (int rc = d_refuse_unaligned("dh_distill_combine", stats, saved)) return rc;
   distill_combine_kernel<<<(T + 255) / 256, 256, 0, s>>>((const float4*)stats, R, T, tau, (float*)ce, (float*)kd, (float4*)saved);
   return d_rc("dh_distill_combine", cudaSuccess);
 }
 int dh_distill_bwd(const void* call, const void* saved, const void* g_ce, const void* g_kd, void* out, int64_t out_ld) {
   const DistillCall& c = *(const DistillCall*)call;
   if (int rc = d_refuse("dh_distill_bwd", c)) return rc;
+  if (int rc = d_refuse_unaligned("dh_distill_bwd", saved, nullptr)) return rc;
   if (c.T == 0) return 0;
   if (c.f32) d_launch_bwd<float>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);
   else d_launch_bwd<__nv_bfloat16>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);

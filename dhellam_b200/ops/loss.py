@@ -16,7 +16,6 @@ depend on the tensor-parallel size.
 """
 from __future__ import annotations
 
-import math
 import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 
@@ -118,12 +117,13 @@ def vocab_parallel_ce_bwd_(logits, labels, lse, grad_per_token, vocab_start: int
 # ----------------------------------------------------------------------------- distillation from a teacher's top logits
 _TEACHER_TYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 MAX_TEACHER_ENTRIES = 1024
+_MIN_TEMPERATURE, _MAX_TEMPERATURE = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _distill_operands(what, logits, labels, top_ids, top_logits, temperature):
     shape, ids, id_type = logits.shape, top_ids.shape, top_ids.dtype
     if len(shape) == 2 and len(ids) == 2 and ids[0] == shape[0] and top_logits.shape == ids and (id_type is torch.int32 or id_type is torch.int64) \
-            and top_logits.dtype in _TEACHER_TYPES and ids[1] <= MAX_TEACHER_ENTRIES and 0.0 < temperature < math.inf \
+            and top_logits.dtype in _TEACHER_TYPES and ids[1] <= MAX_TEACHER_ENTRIES and _MIN_TEMPERATURE <= temperature <= _MAX_TEMPERATURE \
             and (labels is None or (labels.dtype is torch.int32 and labels.shape == shape[:1])):
         return
     if logits.dim() != 2 or top_ids.dim() != 2 or top_ids.shape[0] != logits.shape[0] or top_logits.shape != top_ids.shape:
@@ -134,8 +134,8 @@ def _distill_operands(what, logits, labels, top_ids, top_logits, temperature):
                          f"{top_ids.shape[1]} of {top_ids.dtype} and {top_logits.dtype}")
     if labels is not None and (labels.shape != logits.shape[:1] or labels.dtype != torch.int32):
         raise ValueError(f"{what}: {logits.shape[0]} int32 labels, got {labels.dtype} {tuple(labels.shape)}")
-    if not (0.0 < temperature < float("inf")):
-        raise ValueError(f"{what}: the temperature is positive and finite, not {temperature}")
+    if not _MIN_TEMPERATURE <= temperature <= _MAX_TEMPERATURE:
+        raise ValueError(f"{what}: the temperature is a positive normal fp32 number, not {temperature}")
 
 
 def _distill_native(what, logits, labels, top_ids, top_logits, *others):
@@ -226,7 +226,8 @@ def vocab_parallel_distill_fwd(logits, labels, top_ids, top_logits, temperature:
     ``logits [T, V/t]`` are the student's (bf16 or fp32), this rank's shard of the vocabulary from ``vocab_start`` on.  ``top_ids [T, K]``
     and ``top_logits [T, K]`` are the ids and logits of the teacher's best entries, the same on every rank; an id outside the
     vocabulary is padding.  With ``q = softmax(top_logits / temperature)`` over a row's entries and the student's ``p = softmax(logits /
-    temperature)`` over the whole vocabulary, ``kd = temperature^2 KL(q || p)``; rows without entries give 0.  ``ce`` is the cross entropy
+    temperature)`` over the whole vocabulary, ``kd = temperature^2 KL(q || p)`` (with the roundings of KL, some 2^-22 of its terms, as many
+    times); rows without entries give 0.  ``ce`` is the cross entropy
     against ``labels [T]`` int32 (0 where the label lies outside the vocabulary), or ``None`` without labels.  A row whose logits are
     all ``-inf`` has neither loss nor gradient.  ``saved`` (pairs of fp32 numbers, as complex64) goes to
     ``vocab_parallel_distill_bwd_``.  The ranks of ``group`` exchange eight numbers a token in one all-gather."""
@@ -292,6 +293,8 @@ def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce
     for t, shape, dtype in ((g_kd, (T,), torch.float32), (g_ce, (T,), torch.float32), (saved, (T, 4), torch.complex64)):
         if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
             raise ValueError(f"{what}: contiguous fp32 gradients [T] and statistics [T, 4] as they were saved, got {t.dtype} {tuple(t.shape)}")
+    if saved.data_ptr() % 16:
+        raise ValueError(f"{what}: statistics that start on 16 bytes")
     if K.use_native(logits):
         labels, top_ids, top_logits = _distill_native(what, logits, labels, top_ids, top_logits, saved, g_ce, g_kd, out)
         call = _distill_call(logits, labels, top_ids, top_logits, vocab_start, 2 ** 31 - 1, temperature, sm_budget)

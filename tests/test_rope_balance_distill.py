@@ -389,3 +389,33 @@ def test_distill_teachers_logits_far_from_zero(teacher, low, tau):
     z, labels, ids, top, g_ce, g_kd = case
     ce, kd, saved = L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
     check_distill(exact, tau, ce, kd, L.vocab_parallel_distill_bwd_(z.clone(), labels, ids, top, saved, g_ce, g_kd, tau), torch.float32)
+
+
+def test_distill_operands_that_no_vector_load_takes_are_refused():
+    """By the C functions, before anything is launched: statistics that do not start on 16 bytes, and temperatures at which an exponent's
+    factor leaves fp32."""
+    from dhellam_b200 import kernels as K
+
+    def call(tau=1.0, T=4):
+        return L._DISTILL_CALL.pack(0, 8, 0, 0, 0, 0, 0, 0, 0, 0, T, 8, 0, 0, 8, 0, 0, tau)
+
+    def refused(why, name, types, *args):
+        return K.proto(name, types)(*args) != 0 and why in K.lib().dh_last_error_string().decode()
+    none = call(T=0)                      # nothing to launch either way
+    for at in (8, 4, 24):
+        assert refused("16 bytes", "dh_distill_fwd", L._DISTILL_FWD, none, 0, 0, at, 0)
+        assert refused("16 bytes", "dh_distill_fwd", L._DISTILL_FWD, none, 0, 0, 0, at)
+        assert refused("16 bytes", "dh_distill_bwd", L._DISTILL_BWD, none, at, 0, 0, 0, 8)
+    for tau in (1e-39, 4e-39, 1e-50, 1e39):
+        none = call(tau, T=0)
+        assert refused("temperature", "dh_distill_fwd", L._DISTILL_FWD, none, 0, 0, 0, 0)
+        assert refused("temperature", "dh_distill_bwd", L._DISTILL_BWD, none, 0, 0, 0, 0, 8)
+    z, labels, ids, top, g_ce, g_kd = distill_case(6, 9, 3)
+    saved = L.vocab_parallel_distill_fwd(z, labels, ids, top)[2]
+    flat = torch.zeros(6 * 4 + 1, dtype=saved.dtype)
+    odd = flat[1:].view(6, 4).copy_(saved)
+    with pytest.raises(ValueError, match="16 bytes"):
+        L.vocab_parallel_distill_bwd_(z, labels, ids, top, odd, g_ce, g_kd)
+    for tau in (1e-39, 4e-39, 1e39):
+        with pytest.raises(ValueError):
+            L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
