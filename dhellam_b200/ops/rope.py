@@ -135,6 +135,52 @@ def _fits(x, lead, d, dtype):
     return x.dim() in (3, 4) and x.shape[:-2] == lead and x.shape[-1] == d and x.dtype == dtype and (x.stride(-1) == 1 or d == 1)
 
 
+def _disjoint(a, b=None):
+    """Whether the heads of ``a`` (and of ``b``, of as many rows in the same memory) are all apart: rows of equal strides in which the heads
+    of both follow one another, inside, between or around the row dimensions.  Unusual strides that no such nesting has count as overlapping."""
+    if a.dim() == 3:                                     # packed rows, the heads of a row within its stride: what a training step has
+        (_, heads, d), (row, step, _) = a.shape, a.stride()
+        end = step * (heads - 1) + d
+        if b is None:
+            if step >= d and end <= row:
+                return True
+        elif step >= d:
+            more, (row_b, step_b, _), at = b.shape[1], b.stride(), (b.data_ptr() - a.data_ptr()) // a.element_size()
+            if row_b == row and step_b >= d and at >= end and at + step_b * (more - 1) + d <= row:
+                return True
+    if a.numel() == 0 or (b is not None and b.numel() == 0):
+        return True
+    rows = sorted((st, n) for st, n in zip(a.stride()[:-2], a.shape[:-2]) if n > 1)
+    steps = [(0, a.stride(-2), a.shape[-2])]
+    if b is not None:
+        size, first = a.element_size(), a.data_ptr()
+        spans = [sum(st * (n - 1) for st, n in zip(x.stride(), x.shape)) * size + size for x in (a, b)]
+        if first + spans[0] <= b.data_ptr() or b.data_ptr() + spans[1] <= first:
+            return True
+        if sorted((st, n) for st, n in zip(b.stride()[:-2], b.shape[:-2]) if n > 1) != rows or (b.data_ptr() - first) % size:
+            return False
+        steps.append(((b.data_ptr() - first) // size, b.stride(-2), b.shape[-2]))
+        steps.sort()
+    for inner in range(len(rows) + 1):                   # row dimensions inside the heads
+        extent, fits = a.shape[-1], True
+        for i in range(len(rows) + 1):
+            if i == inner:
+                if all(n == 1 or st >= extent for _, st, n in steps) and (
+                        len(steps) == 1 or steps[0][0] + steps[0][1] * (steps[0][2] - 1) + extent <= steps[1][0]):
+                    extent += max(at + st * (n - 1) for at, st, n in steps) - steps[0][0]
+                else:                                    # heads of both in turn
+                    starts = sorted(at + st * h for at, st, n in steps for h in range(n))
+                    fits &= all(y - x >= extent for x, y in zip(starts, starts[1:]))
+                    extent += starts[-1] - starts[0]
+            if i < len(rows):
+                st, n = rows[i]
+                fits &= st >= extent
+                extent += st * (n - 1)
+        if fits:
+            return True
+    return False
+
+
 def _check(q, k, positions, freq, out, what):
     lead, d = q.shape[:-2], q.shape[-1] if q.dim() else 0
     if positions.shape != lead or positions.dtype not in (torch.int32, torch.int64):
@@ -148,13 +194,17 @@ def _check(q, k, positions, freq, out, what):
     if out is None:
         return
     for x, o in zip(inputs, out):
-        if o.shape != x.shape or not _fits(o, lead, d, q.dtype) or any(n > 1 and st == 0 for n, st in zip(o.shape, o.stride())):
+        if o.shape != x.shape or not _fits(o, lead, d, q.dtype) or not _disjoint(o):
             raise ValueError(f"{what}: an output has its input's shape and type, room for every row and head and elements side by side")
         in_place = o.data_ptr() == x.data_ptr() and o.stride() == x.stride()
         if not in_place and any(o.untyped_storage().data_ptr() == y.untyped_storage().data_ptr() for y in inputs):
             raise ValueError(f"{what}: an output is its own input or shares no memory with the inputs")
-    if k is not None and out[0].data_ptr() == out[1].data_ptr() and q.numel() and k.numel():
-        raise ValueError(f"{what}: queries and keys have outputs of their own")
+    if k is not None:
+        oq, ok = out
+        # an output that is its own input may still share heads with the other one
+        for a, b in ((oq, ok),) + (() if ok is k else ((oq, k),)) + (() if oq is q else ((q, ok),)):
+            if a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr() and not _disjoint(a, b):
+                raise ValueError(f"{what}: an output shares no heads with the other one, nor with its input")
 
 
 def _strides(x):
@@ -225,7 +275,8 @@ def rope_fwd(q, k, positions, freq, interleaved: bool = False, scale: float = 1.
     ``attn_fwd`` does), bf16 or fp32, any strides with the elements of a head side by side; ``k`` may be ``None``.
     ``positions [T]`` (``[S, B]``) int32 or int64, any value.  ``freq [r / 2]`` fp64 and ``scale`` come from
     ``rope_frequencies``: the first ``r`` elements of every head are rotated, as pairs ``(i, i + r/2)`` or, interleaved,
-    ``(2i, 2i + 1)``; the others are copied.  ``out = (q', k')`` names the outputs, which may be the inputs themselves."""
+    ``(2i, 2i + 1)``; the others are copied.  ``out = (q', k')`` names the outputs, which may be the inputs themselves; they share
+    no heads with one another, nor one's with the other's input."""
     return _turn(q, k, positions, freq, interleaved, scale, out, False, sm_budget, stream, "rope_fwd")
 
 

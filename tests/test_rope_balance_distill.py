@@ -419,3 +419,34 @@ def test_distill_operands_that_no_vector_load_takes_are_refused():
     for tau in (1e-39, 4e-39, 1e39):
         with pytest.raises(ValueError):
             L.vocab_parallel_distill_fwd(z, labels, ids, top, tau)
+
+
+def test_rope_outputs_that_overlap_are_refused():
+    """Outputs that share heads with one another, with themselves or with the other input; layouts in which nothing is shared are taken."""
+    buf, pos, (freq, _) = torch.randn(6, 6, 8), torch.arange(6), R.rope_frequencies(8, 10000.0)
+    room = torch.zeros(400)
+    q, k = torch.randn(6, 3, 8), torch.randn(6, 2, 8)
+    bad = [dict(out=(buf[:, :3], buf[:, 2:4])), dict(out=(buf[:, 1:4], buf[:, :2])), dict(q=buf[:, :3], k=buf[:, 2:4], out=(buf[:, :3], buf[:, 2:4])),
+           dict(q=buf[:, :3], k=buf[:, 2:4], out=(buf[:, :3], torch.zeros(6, 2, 8))), dict(q=buf[:, 1:4], k=buf[:, :2], out=(torch.zeros(6, 3, 8), buf[:, :2])),
+           dict(out=(room.as_strided((6, 3, 8), (24, 4, 1)), k)), dict(out=(room.as_strided((6, 3, 8), (20, 8, 1)), torch.zeros(6, 2, 8))),
+           dict(out=(room.as_strided((6, 3, 8), (24, 8, 1)), room.as_strided((6, 2, 8), (24, 8, 1), 100))),
+           dict(out=(room.as_strided((6, 3, 8), (40, 8, 1)), room.as_strided((6, 2, 8), (32, 8, 1), 24)))]
+    for b in bad:
+        with pytest.raises(ValueError):
+            R.rope_fwd(**(dict(q=q, k=k, positions=pos, freq=freq) | b))
+    want = R.rope_fwd(q, k, pos, freq)
+    block = torch.zeros(7, 6, 8)                                             # heads outermost in memory
+    wide = torch.zeros(6, 8, 8)
+    for out in ((block[:3].transpose(0, 1), block[3:5].transpose(0, 1)), (wide[:, 2:5], wide[:, 5:7]), (wide[:, 4:7], wide[:, 1:3]),
+                (wide[:, 0:6:2], wide[:, 1:4:2]), (block[0:6:2].transpose(0, 1), block[1:5:2].transpose(0, 1))):
+        got = R.rope_fwd(q, k, pos, freq, out=out)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # sequence-first views of [B, heads, S, d]: queries and keys of every batch beside one another
+    store = torch.zeros(2, 5, 3, 8)
+    four = store.permute(2, 0, 1, 3)
+    q4, k4, p4 = q.view(3, 2, 3, 8), k.view(3, 2, 2, 8), pos.view(3, 2)
+    got = R.rope_fwd(q4, k4, p4, freq, out=(four[:, :, :3], four[:, :, 3:]))
+    assert torch.equal(got[0].reshape(6, 3, 8), want[0]) and torch.equal(got[1].reshape(6, 2, 8), want[1])
+    four.copy_(torch.cat([q4, k4], 2))
+    R.rope_fwd(four[:, :, :3], four[:, :, 3:], p4, freq, out=(four[:, :, :3], four[:, :, 3:]))
+    assert torch.equal(store.permute(2, 0, 1, 3)[:, :, :3].reshape(6, 3, 8), want[0])
