@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(BT) router_bwd_kernel(const BalArgs a, const R
     if (id >= 0) { pj = p[id]; dot = dg * g; }
     float sel = pj;
     bal_group_sum<L>(dot, sel);
-    float u = id >= 0 && sel != 0.f ? (dg - dot) / sel : 0.f;
+    float u = id >= 0 ? (dg - dot) / sel : 0.f;          // a sum of 0 has no finite gradient: it shows
     float all = u * pj, bal = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i)

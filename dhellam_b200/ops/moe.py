@@ -129,7 +129,10 @@ def aux_loss(probs, topi, E: int):
 def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0, balance: Optional[Balance] = None, sm_budget: int = 0,
                     stream=None):
     """Gradient with respect to the router logits ``[T,E]`` (fp32): of the gates (``d_gates [T,k]``) and, times ``aux_scale``, of the
-    balance loss.  ``balance`` comes from ``balance_loss_fwd``; without it all tokens count."""
+    balance loss.  ``balance`` comes from ``balance_loss_fwd``; without it all tokens count.
+
+    A choice outside ``[0, E)`` (a token that was dropped there) has no gate and gets no gradient; without a ``balance`` it is an error on
+    the CPU, as of any index.  A row whose chosen probabilities sum to 0 has no finite gradient (NaN or infinities)."""
     if stream is not None:
         operands = (d_gates, probs, topi, gates) + (tuple(balance) if balance is not None else ())
         return K.run_on_stream(stream, operands, lambda: router_topk_bwd(d_gates, probs, topi, gates, E, aux_scale, balance, sm_budget))
@@ -161,10 +164,12 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
                                                       coef.data_ptr() if aux_scale else 0, aux_scale, out.data_ptr()), "dh_router_bwd")
         return out
     valid = (topi >= 0) & (topi < E)
+    if balance is None and not topi.is_cuda and not bool(valid.all()):
+        raise IndexError(f"router_topk_bwd: a choice outside the {E} experts")
     at = torch.where(valid, topi, torch.zeros_like(topi)).long()
     topv_sum = torch.where(valid, probs.gather(1, at), 0.0).sum(-1, keepdim=True)
-    dg = torch.where(valid, d_gates, 0.0)
-    d_topv = torch.where(valid & (topv_sum != 0), (dg - (dg * gates).sum(-1, keepdim=True)) / topv_sum, 0.0)
+    dot = torch.where(valid, d_gates * gates, 0.0).sum(-1, keepdim=True)
+    d_topv = torch.where(valid, (d_gates - dot) / topv_sum, 0.0)
     d_probs = torch.zeros_like(probs)
     d_probs.scatter_add_(1, at, d_topv)
     if aux_scale:

@@ -450,3 +450,20 @@ def test_rope_outputs_that_overlap_are_refused():
     four.copy_(torch.cat([q4, k4], 2))
     R.rope_fwd(four[:, :, :3], four[:, :, 3:], p4, freq, out=(four[:, :, :3], four[:, :, 3:]))
     assert torch.equal(store.permute(2, 0, 1, 3)[:, :, :3].reshape(6, 3, 8), want[0])
+
+
+def test_a_corrupted_router_does_not_train_on_in_silence():
+    """As before there was a kernel: chosen probabilities that sum to 0 give no finite gradient, and without a balance a choice outside the
+    experts is an error of the CPU form."""
+    probs, ids, gates, dg, _ = router_case(6, 5, 2)
+    bal = M.balance_loss_fwd(probs, ids)[2]
+    want = M.router_topk_bwd(dg, probs, ids, gates, 5, 0.3, balance=bal)
+    probs[2, ids[2]] = 0.0
+    for balance in (None, bal):
+        got = M.router_topk_bwd(dg, probs, ids, gates, 5, 0.3, balance=balance)
+        assert bool(torch.isnan(got[2]).any()) and torch.equal(got[3:], want[3:]) and torch.equal(got[:2], want[:2])
+    for bad in (-1, 5):
+        ids[1, 1] = bad
+        for choices in (ids, ids.to(torch.int32)):
+            with pytest.raises((RuntimeError, IndexError)):
+                M.router_topk_bwd(dg, probs, choices, gates, 5)

@@ -609,3 +609,18 @@ def test_distill_teachers_logits_far_from_zero(teacher, low, tau, monkeypatch):
         ce, kd, saved = L.vocab_parallel_distill_fwd(part, labels, ids, top, tau, vocab_start=v0)
         L.vocab_parallel_distill_bwd_(part, labels, ids, top, saved, g_ce, g_kd, tau, vocab_start=v0, out=grad[:, v0:v0 + 2000])
     check_distill(exact, tau, ce, kd, grad, F32)
+
+
+def test_router_gradient_of_chosen_probabilities_that_sum_to_zero():
+    """No finite gradient in that row, by the kernel and by the PyTorch ops; rows without any choice have the balance's alone."""
+    for E in (6, 61, 1100):
+        probs, ids, gates, dg, mask = router_case(40, E, 3, device=DEV)
+        bal = M.balance_loss_fwd(probs, ids, mask)[2]
+        want = M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=bal)
+        probs[7, ids[7]] = 0.0
+        for weight, balance in ((0.3, bal), (0.0, None)):
+            got = M.router_topk_bwd(dg, probs, ids, gates, E, weight, balance=balance)
+            assert bool(torch.isnan(got[7]).any()) and bool(torch.isfinite(got[8:]).all()) and bool(torch.isfinite(got[:7]).all())
+            assert balance is None or torch.equal(got[8:], want[8:])
+        ids[9] = -1
+        assert bool(torch.isfinite(M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=bal)[9]).all())
