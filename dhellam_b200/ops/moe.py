@@ -150,7 +150,7 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
             and isinstance(aux_scale, (int, float)) and _on_kernel(probs, topi, d_gates, gates, mask, coef) \
             and (coef is None or coef.dtype is torch.float32):
         if aux_scale and coef is None:
-            coef = balance_loss_fwd(probs, topi)[2].coef
+            coef = balance_loss_fwd(probs, topi, sm_budget=sm_budget)[2].coef
         if mask is not None and not mask.is_contiguous():
             mask = mask.contiguous()
         if coef is not None and not coef.is_contiguous():

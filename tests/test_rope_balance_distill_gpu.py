@@ -624,3 +624,12 @@ def test_router_gradient_of_chosen_probabilities_that_sum_to_zero():
             assert balance is None or torch.equal(got[8:], want[8:])
         ids[9] = -1
         assert bool(torch.isfinite(M.router_topk_bwd(dg, probs, ids, gates, E, 0.3, balance=bal)[9]).all())
+
+
+def test_router_gradient_without_a_balance_keeps_its_budget(monkeypatch):
+    """The balance that it then counts itself runs on as few SMs."""
+    probs, ids, gates, dg, _ = router_case(30, 8, 2, device=DEV)
+    seen, fwd = [], M.balance_loss_fwd
+    monkeypatch.setattr(M, "balance_loss_fwd", lambda *a, **kw: (seen.append((a, kw)), fwd(*a, **kw))[1])
+    M.router_topk_bwd(dg, probs, ids, gates, 8, 0.3, sm_budget=9)
+    assert len(seen) == 1 and (seen[0][1].get("sm_budget") or (seen[0][0] + (None,) * 4)[3]) == 9
