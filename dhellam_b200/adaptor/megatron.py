@@ -160,6 +160,13 @@ def configs_from_args(args, world_size: int):
     """(ModelConfig, ParallelConfig, TrainConfig) from a Megatron-style namespace."""
     nq = args.num_attention_heads
     groups = args.num_query_groups if (args.group_query_attention and args.num_query_groups) else nq
+    if args.rotary_seq_len_interpolation_factor and args.use_rope_scaling:
+        raise ValueError("--rotary-seq-len-interpolation-factor and --use-rope-scaling are two ways of stretching the same positions: give one")
+    if args.position_embedding_type != "rope" and (args.rotary_seq_len_interpolation_factor or args.use_rope_scaling or args.rotary_interleaved
+                                                   or args.rotary_percent != 1.0):
+        raise ValueError("learned positions are not rotated: --rotary-percent, --rotary-interleaved and the scaling of frequencies do not go with them")
+    if args.distill_data and not args.distill_alpha:
+        raise ValueError("--distill-data names a teacher's entries, but --distill-alpha gives them no share of the loss")
     scaling = ("linear", args.rotary_seq_len_interpolation_factor) if args.rotary_seq_len_interpolation_factor else \
         (args.rope_scaling_type, args.rope_scaling_factor) if args.use_rope_scaling else ("none", 1.0)
     cfg = ModelConfig(

@@ -322,3 +322,29 @@ def test_student_step_on_gpu_matches_the_cpu_engine(family, alpha, tau):
         if err > (0.25 if family == "moe" and ("router" in n or "ln_mlp" in n or "expert" in n) else 8e-2):
             bad.append((n, err))
     assert not bad, bad
+
+
+def test_options_that_contradict_each_other_are_refused(tmp_path):
+    import numpy as np
+    import os
+    import subprocess
+    import sys
+    from dhellam_b200.adaptor.megatron import build_parser, configs_from_args
+    from test_train_cli import ARGS, ROOT
+
+    def parse(*more):
+        return configs_from_args(build_parser().parse_args(["--num-layers", "2", "--bf16", *more]), 1)
+    for more in (["--rotary-seq-len-interpolation-factor", "4", "--use-rope-scaling"], ["--distill-data", "teacher"],
+                 ["--position-embedding-type", "learned_absolute", "--use-rope-scaling"],
+                 ["--position-embedding-type", "learned_absolute", "--rotary-seq-len-interpolation-factor", "2"],
+                 ["--position-embedding-type", "learned_absolute", "--rotary-interleaved"],
+                 ["--position-embedding-type", "learned_absolute", "--rotary-percent", "0.5"]):
+        with pytest.raises(ValueError):
+            parse(*more)
+    parse("--position-embedding-type", "learned_absolute", "--rotary-base", "10000")      # a number without meaning there, as before
+    np.arange(100, dtype=np.int32).tofile(str(tmp_path / "t.bin"))
+    _write_teacher(str(tmp_path / "top"), 100, 6, 50)
+    p = subprocess.run([sys.executable, os.path.join(ROOT, "train.py")] + ARGS + ["--train-iters", "1", "--data-path", str(tmp_path / "t.bin"),
+                       "--distill-top-k", "6", "--distill-data", str(tmp_path / "top")], cwd=str(tmp_path),
+                       env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=300)
+    assert p.returncode != 0 and "--distill-alpha" in p.stderr
