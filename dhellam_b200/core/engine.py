@@ -72,7 +72,15 @@ class Env:
             c, s = rope_table(cfg.seq_length, cfg.head_dim, cfg.rope_theta)
             self.rope_cos, self.rope_sin = c.to(self.device), s.to(self.device)
         self.moe_aux = []             # auxiliary (load-balance) losses of the current step
-        self.moe_counts = []          # choices per expert [E] int32 of every router call of the current step
+
+    @property
+    def moe_aux(self):
+        return self._moe_aux
+
+    @moe_aux.setter
+    def moe_aux(self, losses):
+        # a new list of losses begins new counts: (layer, choices per expert [E] int32) of every router call
+        self._moe_aux, self.moe_counts = losses, []
 
 
 def hand_over(obj, stream):
@@ -324,7 +332,6 @@ class DoubleStrandEngine:
         N = len(mbs)
         self.losses = []
         self.env.moe_aux = []
-        self.env.moe_counts = []
         self.grad_scale = self.loss_scale / N
         self.env.grad_scale = self.grad_scale
         st = self.streams

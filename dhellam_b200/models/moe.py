@@ -45,7 +45,7 @@ def f_router(run):
     if env.training and env.cfg.moe_aux_loss_coeff > 0:
         loss, counts, run.acts["moe_balance"] = M.balance_loss_fwd(probs, topi, getattr(run.mb, "token_mask", None))
         env.moe_aux.append(loss)
-        env.moe_counts.append(counts)
+        env.moe_counts.append((run.layer_index, counts))
     run.v["moe_x"] = x
 
 

@@ -143,9 +143,26 @@ class Trainer:
         return None
 
     def expert_load(self):
-        """Choices per expert ``[E]`` of the last step on this rank, over its router calls (``None`` without a balance loss)."""
-        counts = self.env.moe_counts
-        return torch.stack(counts).sum(0) if counts else None
+        """Choices per expert of the last step on this rank, ``[layers, E]`` in the order of this rank's layers: each has experts of its own
+        (``None`` without a balance loss)."""
+        layers = {}
+        for layer, counts in self.env.moe_counts:
+            layers.setdefault(layer, []).append(counts)
+        return torch.stack([torch.stack(layers[i]).sum(0) for i in sorted(layers)]) if layers else None
+
+    def expert_imbalance(self):
+        """The busiest expert's choices against an even share of the last step's, in the layer where that is most, over all tokens and layers
+        of the job (``None`` without a balance loss).  Every rank calls it."""
+        load = self.expert_load()
+        if load is None:
+            return None
+        load, ps = load.to(torch.float64), self.ps
+        if ps.dp_cp_group is not None:
+            dist.all_reduce(load, group=ps.dp_cp_group)
+        most = (load.amax(1) / load.mean(1).clamp_min(1e-9)).max()
+        if ps.pp > 1:
+            dist.all_reduce(most, op=dist.ReduceOp.MAX, group=ps.pp_group)
+        return float(most)
 
     def close(self):
         """Drops every reference this trainer (and the module-level blackboard) holds to the model,

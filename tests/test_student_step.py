@@ -348,3 +348,62 @@ def test_options_that_contradict_each_other_are_refused(tmp_path):
                        "--distill-top-k", "6", "--distill-data", str(tmp_path / "top")], cwd=str(tmp_path),
                        env=dict(os.environ, PYTHONPATH=ROOT), capture_output=True, text=True, timeout=300)
     assert p.returncode != 0 and "--distill-alpha" in p.stderr
+
+
+def test_expert_load_is_kept_by_layer():
+    """Each layer has its own experts: counts ``[layers, E]`` against the choices of the layers' routers, over micro-batches and both strands;
+    whoever begins a new list of balance losses begins new counts."""
+    from dhellam_b200.config import ParallelConfig, TrainConfig, preset
+    from dhellam_b200.data import synthetic_step_batches
+    from dhellam_b200.ops import moe as M
+    from dhellam_b200.parallel import state as PS
+    from dhellam_b200.trainer import Trainer
+    cfg = preset("tiny-moe", seq_length=16, moe_aux_loss_coeff=0.1)
+    train = TrainConfig(micro_batch_size=2, global_batch_size=6, dtype="fp32")
+    PS.set_state(None)
+    tr = Trainer(cfg, ParallelConfig(), train, device="cpu")
+    assert tr.expert_load() is None
+    seen, fwd = [], M.router_topk_fwd
+    try:
+        M.router_topk_fwd = lambda x, w, k: (lambda r: (seen.append((w.data_ptr(), r[1])), r)[1])(fwd(x, w, k))
+        for step in range(2):
+            seen.clear()
+            tr.optimizer.zero_grad()
+            tr.engine.run_step(synthetic_step_batches(cfg, train, tr.ps, step, "cpu"))
+            assert len(seen) == 3 * cfg.num_layers
+            want = torch.zeros(cfg.num_layers, cfg.num_experts, dtype=torch.int64)
+            where = {}
+            for j, (first, second) in enumerate(tr.model.blocks):
+                where[first.router_weight.data_ptr()], where[second.router_weight.data_ptr()] = j, cfg.num_layers - 1 - j
+            for at, topi in seen:
+                want[where[at]] += torch.bincount(topi.reshape(-1), minlength=cfg.num_experts)
+            load = tr.expert_load()
+            assert load.shape == want.shape and torch.equal(load.long(), want)
+    finally:
+        M.router_topk_fwd = fwd
+    tr.env.moe_aux = []
+    assert tr.env.moe_counts == [] and tr.expert_load() is None
+
+
+def _imbalance(rank, world, par):
+    from dhellam_b200.config import ParallelConfig, TrainConfig, preset
+    from dhellam_b200.data import synthetic_step_batches
+    from dhellam_b200.trainer import Trainer
+    import torch.distributed as dist
+    cfg = preset("tiny-moe", seq_length=16, moe_aux_loss_coeff=0.1, num_layers=4)
+    pcfg = ParallelConfig(**par)
+    tr = Trainer(cfg, pcfg, TrainConfig(micro_batch_size=1, global_batch_size=2 * pcfg.dp, dtype="fp32"), device="cpu")
+    train = tr.train
+    tr.optimizer.zero_grad()
+    tr.engine.run_step(synthetic_step_batches(cfg, train, tr.ps, 0, "cpu"))
+    mine = tr.expert_load()
+    assert mine.shape == (cfg.num_layers // pcfg.pp, cfg.num_experts)
+    every = [torch.empty_like(mine) for _ in range(world)]
+    dist.all_gather(every, mine)
+    load = (torch.stack(every).sum(0) if pcfg.pp == 1 else torch.cat(every)).double()
+    assert math.isclose(tr.expert_imbalance(), float((load.amax(1) / load.mean(1)).max()), rel_tol=1e-12)
+
+
+@pytest.mark.parametrize("par", [dict(dp=2, ep=2), dict(cp=2), dict(pp=2)], ids=["dp2", "cp2", "pp2"])
+def test_expert_imbalance_over_ranks(par):
+    run_ranks(_imbalance, 2, par)

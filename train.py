@@ -138,9 +138,9 @@ def _loop(args, tr, train, cfg, pcfg, dataset, device, cuda, start, ml, hb, gate
             ms = float(t)
         lv = float(loss) if loss is not None else None
         extra = {"pp_bubble_ms": tr.engine.pp_bubble_ms()} if tr.engine.time_pp else {}
-        load = tr.expert_load()
-        if load is not None:               # the busiest expert's share against an even one
-            extra["expert_load_max_over_mean"] = float(load.max() / load.float().mean().clamp_min(1e-9))
+        imbalance = tr.expert_imbalance()
+        if imbalance is not None:
+            extra["expert_load_max_over_mean"] = imbalance
         rec = ml.log(it + 1, ms, lv, float(tr.last_grad_norm) if tr.last_grad_norm is not None else None, extra)
         if (it + 1) % train.log_interval == 0:
             print_rank0(f" iteration {it + 1:6d}/{train.train_iters} | elapsed time per iteration (ms): {ms:.1f} | lm loss: "
