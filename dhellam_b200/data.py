@@ -48,9 +48,11 @@ def synthetic_teacher(cfg: ModelConfig, batch: int, k: int, seed: int):
     return ids.to(torch.int32), logits.to(torch.float16)
 
 
-def make_microbatch(cfg: ModelConfig, ps, sample: torch.Tensor, index: int, seed: int, device, pin: bool = False, teacher=None) -> MicroBatch:
+def make_microbatch(cfg: ModelConfig, ps, sample: torch.Tensor, index: int, seed: int, device, pin: bool = False, teacher=None,
+                    token_mask=None) -> MicroBatch:
     """Builds this rank's micro-batch from ``sample [B, S+1]`` (tokens; labels are the shift by one) and, for distillation, the teacher's
-    ``(ids, logits)``, each ``[B, S, K]``: its best entries for the token that follows each position."""
+    ``(ids, logits)``, each ``[B, S, K]``: its best entries for the token that follows each position.  ``token_mask [B, S]`` is 0 on padding,
+    which counts neither in the loss nor in the router's balance (synthetic samples and token files have none)."""
     B = sample.shape[0]
     pos = cp_chunk_positions(cfg.seq_length, ps.cp, ps.cp_rank)
     tok = sample[:, :-1][:, pos.long()]          # [B, S_local]
@@ -58,21 +60,29 @@ def make_microbatch(cfg: ModelConfig, ps, sample: torch.Tensor, index: int, seed
     tokens = tok.t().contiguous().reshape(-1).to(torch.int32)       # sequence-first rows
     labels = lab.t().contiguous().reshape(-1).to(torch.int32)
     positions = pos[:, None].expand(-1, B).contiguous().reshape(-1)
-    mask = torch.ones(tokens.numel(), dtype=torch.float32)
     T = tokens.numel()
+    mask = torch.ones(T, dtype=torch.float32)
+    if token_mask is not None:
+        if token_mask.shape != (B, cfg.seq_length):
+            raise ValueError(f"a token mask of {B} samples of {cfg.seq_length} tokens, got {tuple(token_mask.shape)}")
+        token_mask = token_mask[:, pos.long()].t().reshape(-1) != 0
+        mask = token_mask.to(torch.float32)
     lo, hi = ps.tp_rank * (T // ps.tp), (ps.tp_rank + 1) * (T // ps.tp)
     dev = torch.device(device)
     host = [tokens, labels, mask, positions]
     if teacher is not None:
         host += [t[:, pos.long()].transpose(0, 1).reshape(T, -1).contiguous() for t in teacher]
+    if token_mask is not None:
+        host.append(token_mask)
     if dev.type == "cuda":
         if pin:
             host = [t.pin_memory() for t in host]
         host = [t.to(dev, non_blocking=True) for t in host]
     tokens, labels, mask, positions = host[:4]
-    teacher_ids, teacher_logits = host[4:] if teacher is not None else (None, None)
+    teacher_ids, teacher_logits = host[4:6] if teacher is not None else (None, None)
     return MicroBatch(index=index, tokens=tokens, labels=labels, loss_mask=mask, positions=positions, batch=B, seed=seed,
-                      positions_local=positions[lo:hi], teacher_ids=teacher_ids, teacher_logits=teacher_logits)
+                      positions_local=positions[lo:hi], teacher_ids=teacher_ids, teacher_logits=teacher_logits,
+                      token_mask=host[-1] if token_mask is not None else None)
 
 
 def synthetic_step_batches(cfg: ModelConfig, train: TrainConfig, ps, step: int, device) -> List[MicroBatch]:

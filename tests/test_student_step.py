@@ -407,3 +407,37 @@ def _imbalance(rank, world, par):
 @pytest.mark.parametrize("par", [dict(dp=2, ep=2), dict(cp=2), dict(pp=2)], ids=["dp2", "cp2", "pp2"])
 def test_expert_imbalance_over_ranks(par):
     run_ranks(_imbalance, 2, par)
+
+
+def _padded(rank, world, par, dtype):
+    """A batch whose samples end in padding, on this rank's share of the sequence, against counting by hand."""
+    from dhellam_b200.config import ParallelConfig, TrainConfig, preset
+    from dhellam_b200.data import cp_chunk_positions, make_microbatch, synthetic_tokens
+    from dhellam_b200.parallel import state as PS
+    from dhellam_b200.trainer import Trainer
+    cfg = preset("tiny-moe", seq_length=16, moe_aux_loss_coeff=0.1)
+    pcfg = ParallelConfig(**par)
+    if world == 1:
+        PS.set_state(None)
+    tr = Trainer(cfg, pcfg, TrainConfig(micro_batch_size=3, global_batch_size=3 * pcfg.dp, dtype="fp32"), device="cpu")
+    lengths = torch.tensor([16, 5, 11])
+    mask = (torch.arange(16) < lengths[:, None]).to(dtype)
+    mb = make_microbatch(cfg, tr.ps, synthetic_tokens(cfg, 3, 0), 0, 0, "cpu", token_mask=mask)
+    mine = mask[:, cp_chunk_positions(16, pcfg.cp, tr.ps.cp_rank).long()].t().reshape(-1) != 0
+    assert mb.token_mask.dtype == torch.bool and torch.equal(mb.token_mask, mine) and torch.equal(mb.loss_mask.reshape(-1), mine.float())
+    tr.optimizer.zero_grad()
+    tr.engine.run_step([mb])
+    assert int(tr.expert_load().sum()) == cfg.num_layers * int(mine.sum()) * cfg.moe_top_k
+    assert make_microbatch(cfg, tr.ps, synthetic_tokens(cfg, 3, 0), 0, 0, "cpu").token_mask is None
+    for bad in (mask[:2], mask[:, :8], mask.float().t()):
+        with pytest.raises(ValueError):
+            make_microbatch(cfg, tr.ps, synthetic_tokens(cfg, 3, 0), 0, 0, "cpu", token_mask=bad)
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8, torch.int64, torch.float32])
+def test_padding_reaches_the_loss_and_the_balance(dtype):
+    _padded(0, 1, {}, dtype)
+
+
+def test_padding_reaches_the_loss_and_the_balance_of_context_parallel_ranks():
+    run_ranks(_padded, 2, dict(cp=2), torch.bool)
