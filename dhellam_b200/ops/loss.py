@@ -290,6 +290,8 @@ def vocab_parallel_distill_bwd_(logits, labels, top_ids, top_logits, saved, g_ce
         raise ValueError(f"{what}: logits that are overwritten have room for every row")
     if (g_ce is None) != (labels is None):
         raise ValueError(f"{what}: labels and the gradient of their loss go together")
+    if g_kd is None or saved is None:
+        raise ValueError(f"{what}: the gradient of the distillation loss and the saved statistics are needed")
     for t, shape, dtype in ((g_kd, (T,), torch.float32), (g_ce, (T,), torch.float32), (saved, (T, 4), torch.complex64)):
         if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()):
             raise ValueError(f"{what}: contiguous fp32 gradients [T] and statistics [T, 4] as they were saved, got {t.dtype} {tuple(t.shape)}")

@@ -467,3 +467,11 @@ def test_a_corrupted_router_does_not_train_on_in_silence():
         for choices in (ids, ids.to(torch.int32)):
             with pytest.raises((RuntimeError, IndexError)):
                 M.router_topk_bwd(dg, probs, choices, gates, 5)
+
+
+def test_distill_backward_names_what_is_missing():
+    z, labels, ids, top, g_ce, g_kd = distill_case(6, 9, 3)
+    saved = L.vocab_parallel_distill_fwd(z, labels, ids, top)[2]
+    for s, g in ((None, g_kd), (saved, None)):
+        with pytest.raises(ValueError):
+            L.vocab_parallel_distill_bwd_(z, labels, ids, top, s, g_ce, g)
