@@ -776,6 +776,10 @@ int dh_distill_fwd(const void* call, void* ce, void* kd, void* saved, void* stat
   if (int rc = d_refuse("dh_distill_fwd", c)) return rc;
   if (int rc = d_refuse_unaligned("dh_distill_fwd", saved, stats)) return rc;
   if (c.T == 0) return 0;
+  if (saved == nullptr || (kd == nullptr && stats == nullptr)) {
+    set_last_error_c("dh_distill_fwd", "no place for what a row gives");
+    return (int)cudaErrorInvalidValue;
+  }
   const cudaError_t e = c.f32 ? d_launch_fwd<float>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats)
                               : d_launch_fwd<__nv_bfloat16>(c, (float*)ce, (float*)kd, (float4*)saved, (float4*)stats);
   return d_rc("dh_distill_fwd", e);
@@ -791,6 +795,10 @@ int dh_distill_bwd(const void* call, const void* saved, const void* g_ce, const 
   if (int rc = d_refuse("dh_distill_bwd", c)) return rc;
   if (int rc = d_refuse_unaligned("dh_distill_bwd", saved, nullptr)) return rc;
   if (c.T == 0) return 0;
+  if (saved == nullptr || g_kd == nullptr || out == nullptr || (c.labels != 0 && g_ce == nullptr)) {
+    set_last_error_c("dh_distill_bwd", "no statistics, gradients or output");
+    return (int)cudaErrorInvalidValue;
+  }
   if (c.f32) d_launch_bwd<float>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);
   else d_launch_bwd<__nv_bfloat16>(c, (const float4*)saved, (const float*)g_ce, (const float*)g_kd, out, out_ld);
   return d_rc("dh_distill_bwd", cudaSuccess);

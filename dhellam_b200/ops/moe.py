@@ -164,9 +164,7 @@ def router_topk_bwd(d_gates, probs, topi, gates, E: int, aux_scale: float = 0.0,
                                                       coef.data_ptr() if aux_scale else 0, aux_scale, out.data_ptr()), "dh_router_bwd")
         return out
     valid = (topi >= 0) & (topi < E)
-    if balance is None and not topi.is_cuda and not bool(valid.all()):
-        raise IndexError(f"router_topk_bwd: a choice outside the {E} experts")
-    at = torch.where(valid, topi, torch.zeros_like(topi)).long()
+    at = (topi if balance is None and not topi.is_cuda else torch.where(valid, topi, torch.zeros_like(topi))).long()
     topv_sum = torch.where(valid, probs.gather(1, at), 0.0).sum(-1, keepdim=True)
     dot = torch.where(valid, d_gates * gates, 0.0).sum(-1, keepdim=True)
     d_topv = torch.where(valid, (d_gates - dot) / topv_sum, 0.0)

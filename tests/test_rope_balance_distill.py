@@ -475,3 +475,17 @@ def test_distill_backward_names_what_is_missing():
     for s, g in ((None, g_kd), (saved, None)):
         with pytest.raises(ValueError):
             L.vocab_parallel_distill_bwd_(z, labels, ids, top, s, g_ce, g)
+
+
+def test_distill_calls_without_their_operands_are_refused():
+    """By the C functions, before a kernel could write to or read from nothing."""
+    from dhellam_b200 import kernels as K
+
+    def refused(why, name, types, *args):
+        return K.proto(name, types)(*args) != 0 and why in K.lib().dh_last_error_string().decode()
+    bare, labelled = (L._DISTILL_CALL.pack(16, 8, 0, at, 0, 0, 0, 0, 0, 0, 4, 8, 0, 0, 8, 0, 0, 1.0) for at in (0, 16))
+    assert refused("no place", "dh_distill_fwd", L._DISTILL_FWD, bare, 0, 16, 0, 0)
+    assert refused("no place", "dh_distill_fwd", L._DISTILL_FWD, bare, 0, 0, 0, 16)
+    assert refused("no place", "dh_distill_fwd", L._DISTILL_FWD, bare, 0, 0, 16, 0)
+    for args in ((bare, 0, 0, 16, 16, 8), (bare, 16, 0, 0, 16, 8), (bare, 16, 0, 16, 0, 8), (labelled, 16, 0, 16, 16, 8)):
+        assert refused("no statistics", "dh_distill_bwd", L._DISTILL_BWD, *args)
